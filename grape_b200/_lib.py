@@ -137,6 +137,10 @@ def _declare(lib):
     for name in ("grape_hg1_neg", "grape_hg1_normalise"):
         f(name, [vp, vp], None)
     f("grape_hg1_equal", [vp, vp])
+    f("grape_kv_append", [vp, vp, vp, u32, u32, vp, vp, u32, vp, vp, u64, u32, vp, u64, vp, u64, vp, vp, vp, vp])
+    f("grape_kv_select", [vp, vp, vp, u32, u32, vp, vp, u64, u32, u32, u32, vp, vp])
+    f("grape_kv_attend", [vp, vp, vp, u32, u32, vp, vp, u32, vp, u64, u32, u32, vp, C.c_int32, u32, u32, u64, vp, vp])
+    f("grape_kv_error", [], C.c_char_p)
     for name in _OPTIONAL:
         if hasattr(lib, name):
             f(name, _OPTIONAL[name])

@@ -69,6 +69,7 @@ extern "C" int grape_ctx_destroy(grape_ctx* ctx) {
   cudaStreamSynchronize(ctx->stream);
   if (ctx->g_table) grape_table_destroy(ctx->g_table);
   for (auto& b : ctx->arena) cudaFree(b.ptr);
+  for (auto& b : ctx->kv_work) cudaFree(b.first);
   if (ctx->dstage) cudaFree(ctx->dstage);
   if (ctx->pinned) cudaFreeHost(ctx->pinned);
   if (ctx->d_status) cudaFree(ctx->d_status);

@@ -24,6 +24,9 @@ struct grape_ctx {
   // carves what its kernels need, and the next call on the stream reuses the same memory.
   struct ArenaBlock { void* ptr; size_t size; size_t off; };
   std::vector<ArenaBlock> arena;
+  // workspace of the decode-step calls: grow-only, the last block is the current one.  Outgrown blocks are
+  // kept until the context goes, since a captured graph may still hold their addresses.
+  std::vector<std::pair<void*, size_t>> kv_work;
   // pinned staging buffer for the host-buffer entry points
   void* pinned = nullptr;
   size_t pinned_bytes = 0;
@@ -94,6 +97,9 @@ struct ProfScope {
 constexpr uint32_t STATUS_DIGIT_RANGE = 1u;  // a scalar exceeded the declared max_bits
 constexpr uint32_t STATUS_HIST_RANGE = 2u;   // a lookup query fell outside the table
 constexpr uint32_t STATUS_PIPE_TIMEOUT = 4u; // a bounded wait on a shared-memory copy pipeline ran out
+constexpr uint32_t STATUS_KV_RANGE = 8u;     // a quotient did not fit its type
+constexpr uint32_t STATUS_KV_PLACE = 16u;    // a length, position or page outside the cache, its table or the rotation
+constexpr uint32_t STATUS_KV_EXP = 32u;      // a score outside the exp table, or a row sum of zero
 
 // Every entry point that takes a context makes the context's GPU the calling thread's current
 // device first (allocations and launches would otherwise land on whatever device the caller, or

@@ -362,6 +362,118 @@ int grape_commit_i32_static(const void* d_table, uint32_t n_gens, uint32_t windo
 uint64_t grape_static_scratch_bytes(void);
 const char* grape_static_error(void);
 
+/* ---- decode step over a paged key-value cache ------------------------------------------------- */
+/* The attention half of ONE NEW TOKEN of the quantised model, with every integer tensor its proof
+ * takes: quotients, the remainders that the range lookups check, the arguments and values of the exp
+ * mapping lookup, the softmax.  The reference's model keeps no cache and turns no positions (it proves
+ * whole prompts with one head: zzllama/llama/model.py:166-171,518,543-552); the quantisation rules are
+ * its own (:490-503 quotient and remainder, :543-559 scores, exp table and rounded softmax).
+ * rdiv(x, s) below is the rounded division by 2^s: floor((x + floor(2^s / 2)) / 2^s); the remainder
+ * x - rdiv(x, s) * 2^s lies in [-2^(s-1), 2^(s-1)).
+ * All products and sums are 64-bit integers, so every output is exact and does not depend on how the
+ * work is split; inputs have to keep |q . k| and |x cos| + |x sin| below 2^63.  A quotient that does not
+ * fit its type is stored as the type's nearest value and sets a status bit (grape_ctx_status).
+ * Device data (lengths, page numbers, positions) is checked on the device: what points outside the
+ * cache, the table or the rotation is skipped and sets a status bit, nothing is read or written there.
+ *
+ * A cache is the caller's memory: d_k and d_v hold n_pages pages of page_size slots for kv_heads heads of
+ * head_dim int16 or int32 values (bits 16 or 32); element (page, head, slot, channel) is at
+ * page * page_stride + head * head_stride + slot * slot_stride + channel, in elements, the same for both.
+ * d_bounds (may be NULL) is dense [n_pages][kv_heads][2][head_dim] in the cache's type: per page and
+ * channel the least and the greatest key written since the page's slot 0 was written last.
+ * head_dim: a multiple of 8 up to 4096; strides multiples of 8; page_size up to 4096; pointers on 16 bytes.
+ * A sequence's pages are row b of d_table, int32 [batch][table_width]: position p lies in page
+ * d_table[b][p / page_size], slot p % page_size.
+ * The calls keep their workspace in the context.  A call that needs more than any before it allocates;
+ * inside a stream capture that is refused (GRAPE_ERR_NOMEM), so make one such call before capturing.
+ * Memory handed to a captured graph stays valid until the context is destroyed; graphs of one context
+ * share it, so replay them one after another, as all calls of a context run. */
+typedef struct grape_kv_cache {
+  void* d_k;
+  void* d_v;
+  void* d_bounds;
+  uint64_t page_stride, head_stride, slot_stride;
+  uint32_t n_pages, page_size, kv_heads, head_dim;
+  uint32_t bits;
+  uint32_t k_shift, v_shift; /* keys and values are divided by 2^shift when they are appended */
+} grape_kv_cache;
+
+/* Position rotation of the first `dim` channels (a multiple of 8; 0 = none): d_cos and d_sin are int32
+ * [positions][dim / 2] at scale 2^shift.  Pair i is channels (2i, 2i+1) when interleaved is 1 (the complex
+ * pairs of LLaMA's own code), (i, i + dim/2) when it is 0. */
+typedef struct grape_kv_rotation {
+  const int32_t* d_cos;
+  const int32_t* d_sin;
+  uint32_t positions, dim, shift, interleaved;
+} grape_kv_rotation;
+
+/* Appends tokens: sequence b, which holds d_start[b] tokens, receives tokens d_offsets[b] ..
+ * d_offsets[b+1]-1 of the `tokens` rows of d_k and d_v (int32 [tokens][kv_heads][head_dim], rows `stride`
+ * elements apart; a row stride is a multiple of 4).  With f = rotation->shift (rotation NULL: f = 0 and no
+ * pair) the pair (x0, x1) at position p becomes (x0 c - x1 s, x1 c + x0 s), other channels x * 2^f, and
+ *   key = rdiv(that, f + k_shift)    value = rdiv(v, v_shift)    query = rdiv(that, f)
+ * Keys and values go to the cache, the optional queries d_q [tokens][heads][head_dim] to d_q_out, the
+ * remainders to d_q_rem / d_k_rem / d_v_rem (dense; any may be NULL).  Slots and bounds of pages that
+ * receive nothing stay as they were.  No two sequences of a call may append to the same page.
+ * f + k_shift and v_shift are at most 30. */
+int grape_kv_append(grape_ctx* ctx, const grape_kv_cache* cache, const int32_t* d_table, uint32_t table_width,
+                    uint32_t batch, const int32_t* d_start, const int32_t* d_offsets, uint32_t tokens,
+                    const grape_kv_rotation* rotation, const int32_t* d_q, uint64_t q_stride, uint32_t heads,
+                    const int32_t* d_k, uint64_t k_stride, const int32_t* d_v, uint64_t v_stride,
+                    int32_t* d_q_out, int32_t* d_q_rem, int32_t* d_k_rem, int32_t* d_v_rem);
+
+/* Chooses n_select pages per sequence and key head for the query d_q [batch][heads][head_dim] (rows
+ * q_stride elements apart) from the bounds alone.  bound(page) = max over the heads that share the key
+ * head of sum_d max(q_d lo_d, q_d hi_d): no key of the page has a larger product with the query, so a
+ * page whose bound lies far enough behind the row's maximum has exp values of zero only.  The `recent`
+ * newest pages (at most n_select) are taken first, then the largest bounds, ties to the lowest page.
+ * d_selected: int32 [batch][kv_heads][n_select], the places in the sequence's row of d_table in ascending
+ * order, -1 behind the last (a sequence of fewer pages).  d_bound (may be NULL): int64
+ * [batch][kv_heads][table_width]; entries behind the last page stay as they were, a page outside the cache
+ * has the least int64.  d_len: int32 [batch], tokens in the cache (0 selects nothing). */
+int grape_kv_select(grape_ctx* ctx, const grape_kv_cache* cache, const int32_t* d_table, uint32_t table_width,
+                    uint32_t batch, const int32_t* d_len, const int32_t* d_q, uint64_t q_stride, uint32_t heads,
+                    uint32_t n_select, uint32_t recent, int32_t* d_selected, int64_t* d_bound);
+
+/* What grape_kv_attend writes beside its output; any pointer may be NULL.  Arrays of a value per score are
+ * int32 [batch][heads][max_keys], d_sum is int64 [batch][heads], d_out_rem int32 [batch][heads][head_dim]. */
+typedef struct grape_kv_witness {
+  int32_t* d_score;
+  int32_t* d_score_rem;
+  int32_t* d_exp_in;
+  int32_t* d_exp_out;
+  int32_t* d_softmax;
+  int64_t* d_sum;
+  int32_t* d_out_rem;
+} grape_kv_witness;
+
+/* Attention of one token per sequence: d_q [batch][heads][head_dim] (rows q_stride elements apart; key
+ * head h * kv_heads / heads for head h), over the first d_len[b] positions, or, with d_selected (int32
+ * [batch][kv_heads][n_select], as grape_kv_select writes it), over the positions of those pages; column i
+ * of a row is position i, or slot i % page_size of selected page i / page_size.  Per row:
+ *   acc = q . k, score = rdiv(acc, score_shift) and its remainder
+ *   exp_in = max(score - the row's largest score, exp_low),  exp_out = d_exp[exp_in - exp_low],  sum of exp_out
+ *   softmax = floor((exp_out * 2^soft_shift + floor(sum / 2)) / sum)
+ *   out = rdiv(sum over the keys of softmax * v, soft_shift) and its remainder
+ * The softmax is rounded with the whole row's sum before it meets the values, as the relation
+ * 2 * 2^soft_shift * e - (2 softmax - 1) * sum in [0, 2 sum] of the proof needs it.
+ * d_exp: exp_len values, not negative, with exp_low <= 0 < exp_low + exp_len.  A score further behind the
+ * maximum than the table reaches takes the first entry, and sets a status bit, as does a row of some length
+ * whose sum is zero (its softmax and output are zero).  score_shift up to 31, soft_shift 1..20.
+ * max_keys bounds the columns of a row: a longer sequence sets a status bit and is cut there.  Columns
+ * that hold no position (behind the length, pages outside the cache) are left as they were and weigh
+ * nothing; a row without any position has output, remainder and sum zero.
+ * d_out: int32 [batch][heads][head_dim]. */
+int grape_kv_attend(grape_ctx* ctx, const grape_kv_cache* cache, const int32_t* d_table, uint32_t table_width,
+                    uint32_t batch, const int32_t* d_len, const int32_t* d_selected, uint32_t n_select,
+                    const int32_t* d_q, uint64_t q_stride, uint32_t heads, uint32_t score_shift,
+                    const int32_t* d_exp, int32_t exp_low, uint32_t exp_len, uint32_t soft_shift,
+                    uint64_t max_keys, int32_t* d_out, const grape_kv_witness* witness);
+
+/* The calling thread's last refusal by one of the three calls above (they check their arguments before
+ * the context, so that a program can have them checked without a GPU: ctx = NULL). */
+const char* grape_kv_error(void);
+
 /* ---- diagnostics and measurement ----------------------------------------------------------- */
 /* Element-wise add (0) / sub (1) / mul (2) over the base field Fp; test hook for the curve code. */
 int grape_fp_binary(grape_ctx* ctx, int op, const void* d_a, const void* d_b, void* d_out, uint64_t n);
@@ -372,7 +484,9 @@ int grape_bls12_381_field_binary(grape_ctx* ctx, int field, int op, const void* 
                                  void* d_out, uint64_t n);
 int grape_bls12_381_fr_from_i32(grape_ctx* ctx, const int32_t* d_in, void* d_out, uint64_t n);
 int grape_bls12_381_measure_mul_peak(grape_ctx* ctx, double* muls_per_second);
-/* Device status word: bit 0 = a scalar exceeded max_bits, bit 1 = lookup query outside its table.
+/* Device status word: bit 0 = a scalar exceeded max_bits, bit 1 = lookup query outside its table,
+ * bit 2 = a bounded wait ran out, bit 3 = a quotient did not fit its type, bit 4 = a length, position or page
+ * outside the cache, its table or the rotation, bit 5 = a score outside the exp table or a row sum of zero.
  * Kernels set bits instead of trapping; reading synchronises and clears. */
 int grape_ctx_status(grape_ctx* ctx, uint32_t* flags);
 /* Kernels launched by this library on the context so far. */
