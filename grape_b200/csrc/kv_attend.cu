@@ -25,7 +25,11 @@ struct AttendArgs {
   int64_t* sum;
   int32_t* chunk_max;  // [batch][heads][chunks]
   int64_t* acc;        // [batch][heads][head_dim]
-  uint32_t chunks, chunk_keys;
+  uint32_t* done;      // blocks of a key head's tile and part that have added to acc
+  uint32_t tiles, split, chunks, chunk_keys;  // scores: head tiles of a key head, warps of a row, blocks of a row
+  uint32_t exp_chunks;
+  uint32_t v_tiles, v_parts, v_split, v_chunks, v_chunk_keys;  // values: head tiles, parts of a row, warps of a part, ...
+  uint32_t done_per_tile;
 };
 
 // Columns of a row that can hold a position: its length, or the slots of the selected pages.
@@ -58,183 +62,581 @@ __device__ __forceinline__ int32_t column_page(const AttendArgs& a, uint32_t b, 
   return page;
 }
 
-constexpr int AT_THREADS = 256;
+// 16 bytes that are read once: past L1.
+__device__ __forceinline__ uint4 load_once(const char* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 
-// Scores of one head over a chunk of columns, a warp a column; the chunk's largest.
+__device__ __forceinline__ void mma_u8s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_u8u8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// ---- scores --------------------------------------------------------------------------------------
+// q . k exactly, on the 8-bit matrix instruction.  k is read as it lies: 4 (or 2) unsigned bytes once its sign
+// bit is flipped (k' = k + bias, bias = 2^31 or 2^15), and q in five balanced digits base 256 (four in
+// [-128, 127] and a fifth of 0 or 1).  Byte p of k' meets digit r of q at weight 256^(p + r), so ONE operand
+// column per weight c, holding digit c - p at byte p, gives
+//   q . k = sum_c 256^c (k' bytes . column c) - bias sum_d q_d,      c = 0 .. 7
+// and the eight weights are the eight columns of an m16n8k32: 16 keys, 32 bytes of each, one head.  A sum
+// of a column is at most 4096 elements x 4 bytes x 255 x 128 < 2^31.
+// A warp takes 16 keys (rows g and g + 8 of a lane), 64 bytes of them per step: a lane's 16 bytes are the A
+// registers of two instructions, no shuffles, no staging.  The columns (8 words per 4 bytes of a key) are
+// built once per block in shared memory.
+// What bounds it: bytes of the keys.  The instruction takes 2 cycles of an SM (measured, 570 T products/s) for
+// 512 bytes of keys and a head, which arrive every 22 cycles.
+constexpr int SC_MAX_THREADS = 512;
+constexpr int SC_SMEM = 128 * 1024;  // columns of a block at most
+
 template <int EB>
-__global__ void __launch_bounds__(AT_THREADS) k_kv_scores(AttendArgs a) {
-  __shared__ int32_t s_max[AT_THREADS / 32];
+__device__ __forceinline__ uint32_t column_word(const uint64_t (&u)[4 / EB], int c) {
+  // u: q + 0x80808080 per element, whose bytes are the digits + 128 and whose fifth byte is the fifth digit
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 4 / EB; e++) {
+#pragma unroll
+    for (int p = 0; p < EB; p++) {
+      const int r = c - p;
+      if (r >= 0 && r <= 4) {
+        uint32_t digit = (uint32_t)(u[e] >> (8 * r)) & 0xffu;
+        if (r < 4) digit ^= 0x80u;
+        w |= digit << (8 * (e * EB + p));
+      }
+    }
+  }
+  return w;
+}
+
+template <int EB, int HT>
+__global__ void __launch_bounds__(SC_MAX_THREADS) k_kv_scores(AttendArgs a) {
+  extern __shared__ uint4 s_w[];  // [blk][HT][32 lanes]: 4 words, the columns of a lane's 16 bytes
+  __shared__ int64_t s_part[SC_MAX_THREADS / 32 * 16 * (HT > 4 ? 4 : HT)];
+  __shared__ unsigned long long s_bias[HT];
+  __shared__ int32_t s_max[HT];
   const KvView& c = a.c;
-  const uint32_t chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, h = row % a.heads, b = row / a.heads, g = h / a.group;
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = c.head_dim;
-  const uint32_t n = kv_length(c, a.len, b, a.selected ? ~0ull : a.max_keys, false), cols = columns(a, b, chunk == 0 && threadIdx.x == 0);
+  const uint32_t D = c.head_dim, row_bytes = D * EB, blks = (row_bytes + 63) / 64;
+  uint32_t x = blockIdx.x;
+  const uint32_t tile = x % a.tiles;
+  x /= a.tiles;
+  const uint32_t chunk = x % a.chunks, row = x / a.chunks, g = row % c.kv_heads, b = row / c.kv_heads;
+  const uint32_t h0 = g * a.group + tile * HT, hn = min((uint32_t)HT, a.group - tile * HT);
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  const uint32_t n = kv_length(c, a.len, b, a.selected ? ~0ull : a.max_keys, false);
+  const uint32_t cols = columns(a, b, chunk == 0 && tid == 0);
+  const uint64_t row0 = (uint64_t)b * a.heads + h0;  // first of the block's rows
   if (chunk == 0) {
-    for (uint32_t d = threadIdx.x; d < D; d += AT_THREADS) a.acc[(uint64_t)row * D + d] = 0;
-    if (threadIdx.x == 0) a.sum[row] = 0;
+    // what the later passes add to
+    for (uint32_t i = tid; i < hn * D; i += blockDim.x) a.acc[row0 * D + i] = 0;
+    for (uint32_t i = tid; i < hn; i += blockDim.x) a.sum[row0 + i] = 0;
+    for (uint32_t i = tid; tile == 0 && i < a.done_per_tile; i += blockDim.x) a.done[(uint64_t)row * a.done_per_tile + i] = 0;
+    if (cols == 0) {
+      for (uint32_t i = tid; i < hn * D; i += blockDim.x) {
+        a.out[row0 * D + i] = 0;
+        if (a.out_rem) a.out_rem[row0 * D + i] = 0;
+      }
+    }
   }
   const uint32_t first = chunk * a.chunk_keys, last = min(cols, first + a.chunk_keys);
-  const int32_t* q = a.q + (uint64_t)b * a.q_stride + (uint64_t)h * D;
-  int32_t best = INT32_MIN;
-  bool range = false;
-  for (uint32_t i = first + warp; i < last; i += AT_THREADS / 32) {
-    uint32_t slot;
-    const int32_t page = column_page(a, b, g, n, i, slot, lane == 0);
-    if (page < 0) continue;
-    const char* k = c.k + page * c.page_stride + g * c.head_stride + slot * c.slot_stride;
-    int64_t acc = 0;
-    for (uint32_t d = lane * 4; d < D; d += 128) {
-      const int4 x = __ldg(reinterpret_cast<const int4*>(q + d));
-      int4 y;
-      if (EB == 4) {
-        y = __ldg(reinterpret_cast<const int4*>(k + d * 4));
-      } else {
-        const short4 s = __ldg(reinterpret_cast<const short4*>(k + d * 2));
-        y = make_int4(s.x, s.y, s.z, s.w);
+  if (first >= last) return;
+
+  if (tid < HT) { s_bias[tid] = 0; s_max[tid] = INT32_MIN; }
+  __syncthreads();
+  const int32_t* q = a.q + (uint64_t)b * a.q_stride + (uint64_t)h0 * D;
+  constexpr uint32_t PER = 4 / EB;  // elements of a word
+  for (uint32_t h = 0; h < HT; h++) {
+    int64_t total = 0;
+    for (uint32_t i = tid; i < blks * 16; i += blockDim.x) {
+      uint64_t u[PER];
+#pragma unroll
+      for (uint32_t e = 0; e < PER; e++) {
+        const uint32_t d = i * PER + e;
+        const int32_t v = h < hn && d < D ? __ldg(q + (uint64_t)h * D + d) : 0;
+        total += v;
+        u[e] = (uint64_t)((int64_t)v + 0x80808080ll);
       }
-      acc += (int64_t)x.x * y.x + (int64_t)x.y * y.y + (int64_t)x.z * y.z + (int64_t)x.w * y.w;
+      // word i of the row: block i / 16, lane group (i / 4) % 4, word i % 4
+      uint32_t* to = reinterpret_cast<uint32_t*>(s_w + ((uint64_t)(i / 16) * HT + h) * 32 + (i / 4) % 4) + i % 4;
+#pragma unroll
+      for (int k = 0; k < 8; k++) to[k * 16] = column_word<EB>(u, k);
     }
-    for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(~0u, acc, o);
-    const int64_t s = rdiv(acc, a.score_shift);
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+    if (lane == 0) atomicAdd(&s_bias[h], (unsigned long long)total);
+  }
+  __syncthreads();
+
+  const uint32_t gl = lane >> 2, t = lane & 3;
+  const uint32_t wd = warp % a.split, wk = warp / a.split, keys_at_once = warps / a.split * 16;
+  const uint32_t blk0 = blks * wd / a.split, blk1 = blks * (wd + 1) / a.split;
+  const uint64_t bias = EB == 4 ? uint64_t(1) << 31 : uint64_t(1) << 15;
+  constexpr uint32_t FLIP = EB == 4 ? 0x80000000u : 0x80008000u;
+  int32_t best[HT];
+#pragma unroll
+  for (int h = 0; h < HT; h++) best[h] = INT32_MIN;
+  bool range = false;
+  auto finish = [&](uint64_t acc, uint32_t h, uint32_t i) {
+    acc -= bias * (uint64_t)s_bias[h];
+    const int64_t s = rdiv((int64_t)acc, a.score_shift);
     const int32_t v = saturate(s, INT32_MIN, INT32_MAX, range);
-    best = max(best, v);
-    if (lane == 0) {
-      const uint64_t at = (uint64_t)row * a.max_keys + i;
-      a.score[at] = v;
-      if (a.score_rem) a.score_rem[at] = (int32_t)(uint32_t)((uint64_t)acc - ((uint64_t)s << a.score_shift));
+    const uint64_t at = (row0 + h) * a.max_keys + i;
+    a.score[at] = v;
+    if (a.score_rem) a.score_rem[at] = (int32_t)(uint32_t)(acc - ((uint64_t)s << a.score_shift));
+    return v;
+  };
+
+  for (uint32_t base = first; base < last; base += keys_at_once) {
+    const uint32_t i0 = base + wk * 16 + gl, i1 = i0 + 8;
+    const char* k0 = nullptr;
+    const char* k1 = nullptr;
+    uint32_t slot;
+    if (i0 < last) {
+      const int32_t page = column_page(a, b, g, n, i0, slot, t == 0 && wd == 0);
+      if (page >= 0) k0 = c.k + page * c.page_stride + g * c.head_stride + slot * c.slot_stride + t * 16;
+    }
+    if (i1 < last) {
+      const int32_t page = column_page(a, b, g, n, i1, slot, t == 0 && wd == 0);
+      if (page >= 0) k1 = c.k + page * c.page_stride + g * c.head_stride + slot * c.slot_stride + t * 16;
+    }
+    int32_t acc[HT][4];
+#pragma unroll
+    for (int h = 0; h < HT; h++) acc[h][0] = acc[h][1] = acc[h][2] = acc[h][3] = 0;
+    constexpr int U = 4;
+    for (uint32_t blk = blk0; blk < blk1; blk += U) {
+      uint4 x0[U], x1[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const bool in = blk + u < blk1 && (blk + u) * 64 + t * 16 < row_bytes;
+        x0[u] = in && k0 ? load_once(k0 + (blk + u) * 64) : make_uint4(0, 0, 0, 0);
+        x1[u] = in && k1 ? load_once(k1 + (blk + u) * 64) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        if (blk + u >= blk1) break;
+        const uint4 y0 = make_uint4(x0[u].x ^ FLIP, x0[u].y ^ FLIP, x0[u].z ^ FLIP, x0[u].w ^ FLIP);
+        const uint4 y1 = make_uint4(x1[u].x ^ FLIP, x1[u].y ^ FLIP, x1[u].z ^ FLIP, x1[u].w ^ FLIP);
+        const uint4* w = s_w + (uint64_t)(blk + u) * HT * 32 + lane;
+#pragma unroll
+        for (int h = 0; h < HT; h++) {
+          if (HT > 2 && h >= hn) break;
+          const uint4 m = w[h * 32];
+          mma_u8s8(acc[h], y0.x, y1.x, y0.y, y1.y, m.x, m.y);
+          mma_u8s8(acc[h], y0.z, y1.z, y0.w, y1.w, m.z, m.w);
+        }
+      }
+    }
+    // lane (g, t) holds columns 2t and 2t + 1 of keys g and g + 8
+#pragma unroll
+    for (int h = 0; h < HT; h++) {
+      uint64_t v0 = ((uint64_t)(int64_t)acc[h][0] + ((uint64_t)(int64_t)acc[h][1] << 8)) << (16 * t);
+      uint64_t v1 = ((uint64_t)(int64_t)acc[h][2] + ((uint64_t)(int64_t)acc[h][3] << 8)) << (16 * t);
+      v0 += __shfl_xor_sync(~0u, v0, 1);
+      v1 += __shfl_xor_sync(~0u, v1, 1);
+      v0 += __shfl_xor_sync(~0u, v0, 2);
+      v1 += __shfl_xor_sync(~0u, v1, 2);
+      if (a.split == 1) {
+        if (t == (h & 3) && h < hn) {
+          if (k0) best[h] = max(best[h], finish(v0, h, i0));
+          if (k1) best[h] = max(best[h], finish(v1, h, i1));
+        }
+      } else {
+        // the warps that share the keys: four heads at a time through shared memory
+        constexpr int AT_ONCE = HT > 4 ? 4 : HT;
+        if (h % AT_ONCE == 0) __syncthreads();
+        if (t == 0) {
+          s_part[(warp * AT_ONCE + h % AT_ONCE) * 16 + gl] = (int64_t)v0;
+          s_part[(warp * AT_ONCE + h % AT_ONCE) * 16 + gl + 8] = (int64_t)v1;
+        }
+        if (h % AT_ONCE == AT_ONCE - 1) {
+          __syncthreads();
+          // warp wd of a group adds the heads wd, wd + split, ...: lanes 0..15 the group's 16 keys, whose validity
+          // lane (gl, t) knows for keys gl and gl + 8
+          const uint32_t valid = __ballot_sync(~0u, k0 != nullptr && t == 0), valid1 = __ballot_sync(~0u, k1 != nullptr && t == 0);
+#pragma unroll
+          for (int j = 0; j < AT_ONCE; j++) {
+            const int hh = h - (AT_ONCE - 1) + j;
+            if (j % a.split == wd && hh < hn && lane < 16) {
+              const bool ok = ((lane < 8 ? valid : valid1) >> ((lane & 7) * 4)) & 1;
+              uint64_t v = 0;
+              for (uint32_t w2 = 0; w2 < a.split; w2++) v += (uint64_t)s_part[((wk * a.split + w2) * AT_ONCE + j) * 16 + lane];
+              if (ok) best[hh] = max(best[hh], finish(v, hh, base + wk * 16 + lane));
+            }
+          }
+        }
+      }
     }
   }
   if (range) kv_flag(c, STATUS_KV_RANGE);
-  if (lane == 0) s_max[warp] = best;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 0; w < AT_THREADS / 32; w++) best = max(best, s_max[w]);
-    a.chunk_max[(uint64_t)row * a.chunks + chunk] = best;
+#pragma unroll
+  for (int h = 0; h < HT; h++) {
+    for (int o = 16; o; o >>= 1) best[h] = max(best[h], __shfl_xor_sync(~0u, best[h], o));
+    if (lane == 0) atomicMax(&s_max[h], best[h]);
   }
+  __syncthreads();
+  if (tid < hn) a.chunk_max[(row0 + tid) * a.chunks + chunk] = s_max[tid];
 }
 
-__global__ void __launch_bounds__(AT_THREADS) k_kv_exp(AttendArgs a) {
-  __shared__ int32_t s_max;
-  __shared__ unsigned long long s_sum;
+// ---- exp -----------------------------------------------------------------------------------------
+// exp_in, exp_out and the row's sum; V columns of a row per thread (4 where they share a page and 16 bytes).
+constexpr int EX_THREADS = 256;
+constexpr uint32_t EX_KEYS = 2048;  // columns of a block
+
+template <int V>
+__global__ void __launch_bounds__(EX_THREADS) k_kv_exp(AttendArgs a) {
+  __shared__ int32_t s_max[EX_THREADS / 32];
+  __shared__ int64_t s_sum[EX_THREADS / 32];
   const KvView& c = a.c;
-  const uint32_t chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, h = row % a.heads, b = row / a.heads, g = h / a.group;
+  const uint32_t chunk = blockIdx.x % a.exp_chunks, row = blockIdx.x / a.exp_chunks, h = row % a.heads, b = row / a.heads, g = h / a.group;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t n = kv_length(c, a.len, b, a.selected ? ~0ull : a.max_keys, false), cols = columns(a, b, false);
-  const uint32_t first = chunk * a.chunk_keys, last = min(cols, first + a.chunk_keys);
+  const uint32_t first = chunk * EX_KEYS, last = min(cols, first + EX_KEYS);
   if (first >= last) return;
-  if (threadIdx.x == 0) { s_max = INT32_MIN; s_sum = 0; }
+  int32_t best = INT32_MIN;
+  const uint32_t used = (cols + a.chunk_keys - 1) / a.chunk_keys;
+  for (uint32_t i = threadIdx.x; i < used; i += EX_THREADS) best = max(best, a.chunk_max[(uint64_t)row * a.chunks + i]);
+  for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
+  if (lane == 0) s_max[warp] = best;
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < a.chunks; i += AT_THREADS) atomicMax(&s_max, a.chunk_max[(uint64_t)row * a.chunks + i]);
-  __syncthreads();
-  const int64_t top = s_max;
+  for (int w = 0; w < EX_THREADS / 32; w++) best = max(best, s_max[w]);
+  const int64_t top = best;
   int64_t sum = 0;
   bool outside = false;
-  for (uint32_t i = first + threadIdx.x; i < last; i += AT_THREADS) {
+  for (uint32_t i = first + threadIdx.x * V; i < last; i += EX_THREADS * V) {
     uint32_t slot;
     if (column_page(a, b, g, n, i, slot, false) < 0) continue;
     const uint64_t at = (uint64_t)row * a.max_keys + i;
-    int64_t x = a.score[at] - top;
-    if (x < a.exp_low) { x = a.exp_low; outside = true; }
-    int32_t e = __ldg(a.exp + (x - a.exp_low));
-    if (e < 0) { e = 0; outside = true; }
-    if (a.exp_in) a.exp_in[at] = (int32_t)x;
-    a.exp_out[at] = e;
-    sum += e;
+    // how many of the V columns hold a position: the page's last tokens may end inside
+    uint32_t m = V;
+    if (V > 1) {
+      m = min(m, last - i);
+      for (uint32_t j = 1; j < m; j++)
+        if (column_page(a, b, g, n, i + j, slot, false) < 0) { m = j; break; }
+    }
+    int32_t s[V], x[V], e[V];
+    if (V == 4 && m == 4) {
+      const int4 v = *reinterpret_cast<const int4*>(a.score + at);
+      s[0] = v.x; s[1 % V] = v.y; s[2 % V] = v.z; s[3 % V] = v.w;
+    } else {
+      for (uint32_t j = 0; j < V; j++) s[j] = j < m ? a.score[at + j] : (int32_t)top;
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const int64_t d = s[j] - top;
+      if (d < a.exp_low) outside = true;
+      x[j] = (int32_t)max(d, (int64_t)a.exp_low);
+      e[j] = __ldg(a.exp + (x[j] - a.exp_low));
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      if (e[j] < 0) { e[j] = 0; outside = true; }
+      if (j < m) sum += e[j];
+    }
+    if (V == 4 && m == 4) {
+      if (a.exp_in) *reinterpret_cast<int4*>(a.exp_in + at) = make_int4(x[0], x[1 % V], x[2 % V], x[3 % V]);
+      *reinterpret_cast<int4*>(a.exp_out + at) = make_int4(e[0], e[1 % V], e[2 % V], e[3 % V]);
+    } else {
+      for (uint32_t j = 0; j < m; j++) {
+        if (a.exp_in) a.exp_in[at + j] = x[j];
+        a.exp_out[at + j] = e[j];
+      }
+    }
   }
   if (outside) kv_flag(c, STATUS_KV_EXP);
-  atomicAdd(&s_sum, (unsigned long long)sum);
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) atomicAdd(reinterpret_cast<unsigned long long*>(a.sum + row), s_sum);
-}
-
-// Softmax of a chunk and its part of the output, a thread four channels.
-template <int EB>
-__global__ void __launch_bounds__(AT_THREADS) k_kv_values(AttendArgs a) {
-  __shared__ int32_t s_o[AT_THREADS];
-  __shared__ int64_t s_at[AT_THREADS];
-  const KvView& c = a.c;
-  const uint32_t chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, h = row % a.heads, b = row / a.heads, g = h / a.group;
-  const uint32_t D = c.head_dim;
-  const uint32_t n = kv_length(c, a.len, b, a.selected ? ~0ull : a.max_keys, false), cols = columns(a, b, false);
-  const uint32_t first = chunk * a.chunk_keys, last = min(cols, first + a.chunk_keys);
-  if (first >= last) return;
-  const int64_t sum = a.sum[row];
-  for (uint32_t base = first; base < last; base += AT_THREADS) {
-    const uint32_t i = base + threadIdx.x;
-    uint32_t slot = 0;
-    const int32_t page = i < last ? column_page(a, b, g, n, i, slot, false) : -1;
-    int32_t o = 0;
-    if (page >= 0) {
-      const uint64_t at = (uint64_t)row * a.max_keys + i;
-      if (sum > 0) o = (int32_t)((((int64_t)a.exp_out[at] << a.soft_shift) + sum / 2) / sum);
-      if (a.softmax) a.softmax[at] = o;
-    }
-    __syncthreads();
-    s_o[threadIdx.x] = o;
-    s_at[threadIdx.x] = page >= 0 ? page * c.page_stride + g * c.head_stride + slot * c.slot_stride : -1;
-    __syncthreads();
-    const uint32_t m = min((uint32_t)AT_THREADS, last - base);
-    for (uint32_t d = threadIdx.x * 4; d < D; d += AT_THREADS * 4) {
-      int64_t acc[4] = {};
-      for (uint32_t j = 0; j < m; j++) {
-        if (s_at[j] < 0 || s_o[j] == 0) continue;
-        int4 y;
-        if (EB == 4) {
-          y = __ldg(reinterpret_cast<const int4*>(c.v + s_at[j] + d * 4));
-        } else {
-          const short4 s = __ldg(reinterpret_cast<const short4*>(c.v + s_at[j] + d * 2));
-          y = make_int4(s.x, s.y, s.z, s.w);
-        }
-        const int64_t w = s_o[j];
-        acc[0] += w * y.x;
-        acc[1] += w * y.y;
-        acc[2] += w * y.z;
-        acc[3] += w * y.w;
-      }
-      for (int j = 0; j < 4; j++) atomicAdd(reinterpret_cast<unsigned long long*>(a.acc + (uint64_t)row * D + d + j), (unsigned long long)acc[j]);
-    }
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < EX_THREADS / 32; w++) sum += s_sum[w];
+    atomicAdd(reinterpret_cast<unsigned long long*>(a.sum + row), (unsigned long long)sum);
   }
 }
 
-__global__ void __launch_bounds__(AT_THREADS) k_kv_out(AttendArgs a, uint64_t total) {
-  const uint64_t i = (uint64_t)blockIdx.x * AT_THREADS + threadIdx.x;
-  if (i >= total) return;
-  const uint64_t row = i / a.c.head_dim;
+// ---- values ----------------------------------------------------------------------------------------
+// sum_j o_j v_j exactly, on the same instruction.  o is at most 2^20: three unsigned digits base 256, which are
+// the operand columns (3 per head); the rows are the bytes of v (v' = v + bias unsigned), so that
+//   sum_j o_j v_j = sum_p,r 256^(p + r) (byte plane p of v' . digit r of o) - bias sum_j o_j.
+// A warp takes 32 keys x 128 bytes of their rows: lane (g, t) loads 16 bytes of the 8 keys 8t .. 8t+7, and
+// turning 4 keys x 4 bytes in registers (8 byte permutes) gives the A registers, keys along the instruction's
+// inner dimension.  Sums of a chunk of at most 16384 keys stay below 16384 x 255 x 255 < 2^31.
+constexpr int VA_THREADS = 256;
+constexpr uint32_t VA_KEYS = 256;          // keys whose softmax a block holds at a time
+constexpr uint32_t VA_STRIDE = VA_KEYS + 32;  // of a column's digits: eight columns on different banks
+constexpr uint32_t VA_MAX_CHUNK = 16384;
+
+// bytes [key][plane] of 4 words -> words [plane] of 4 keys
+__device__ __forceinline__ void turn4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&o)[4]) {
+  const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
+  const uint32_t cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
+  o[0] = __byte_perm(ab0, cd0, 0x5410);
+  o[1] = __byte_perm(ab0, cd0, 0x7632);
+  o[2] = __byte_perm(ab1, cd1, 0x5410);
+  o[3] = __byte_perm(ab1, cd1, 0x7632);
+}
+
+template <int EB, int HT>
+__global__ void __launch_bounds__(VA_THREADS) k_kv_values(AttendArgs a) {
+  constexpr int NT = (3 * HT + 7) / 8;       // instruction columns in eights
+  constexpr uint32_t ELEMS = 128 / EB;       // channels of a warp
+  constexpr uint32_t DIGITS = VA_STRIDE * 8 * NT, PART = VA_THREADS / 32 * 8 * ELEMS * 8;
+  __shared__ __align__(16) unsigned char s_raw[DIGITS > PART ? DIGITS : PART];  // digits [column][key], later partial sums
+  __shared__ __align__(16) int64_t s_at[VA_KEYS];
+  __shared__ unsigned long long s_total[HT];
+  __shared__ uint32_t s_last;
+  const KvView& c = a.c;
+  const uint32_t D = c.head_dim, row_bytes = D * EB, segments = (row_bytes + 127) / 128;
+  uint32_t x = blockIdx.x;
+  const uint32_t tile = x % a.v_tiles;
+  x /= a.v_tiles;
+  const uint32_t part = x % a.v_parts;
+  x /= a.v_parts;
+  const uint32_t chunk = x % a.v_chunks, row = x / a.v_chunks, g = row % c.kv_heads, b = row / c.kv_heads;
+  const uint32_t h0 = g * a.group + tile * HT, hn = min((uint32_t)HT, a.group - tile * HT);
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t = lane & 3;
+  const uint32_t n = kv_length(c, a.len, b, a.selected ? ~0ull : a.max_keys, false), cols = columns(a, b, false);
+  const uint32_t first = chunk * a.v_chunk_keys, last = min(cols, first + a.v_chunk_keys);
+  if (first >= last) return;
+  const uint64_t row0 = (uint64_t)b * a.heads + h0;
+  const uint32_t wd = warp % a.v_split, wk = warp / a.v_split, groups = VA_THREADS / 32 / a.v_split;
+  const uint32_t segment = part * a.v_split + wd, byte = segment * 128 + gl * 16;
+  const bool in_row = segment < segments && byte < row_bytes;
+  if (tid < HT) s_total[tid] = 0;
+  int32_t acc[8][NT][4];
+#pragma unroll
+  for (int m = 0; m < 8; m++)
+#pragma unroll
+    for (int k = 0; k < NT; k++) acc[m][k][0] = acc[m][k][1] = acc[m][k][2] = acc[m][k][3] = 0;
+
+  for (uint32_t base = first; base < last; base += VA_KEYS) {
+    __syncthreads();
+    // the softmax of the next keys, a thread a key
+    {
+      static_assert(VA_KEYS == VA_THREADS, "a thread a key");
+      const uint32_t i = base + tid;
+      uint32_t slot = 0;
+      const int32_t page = i < last ? column_page(a, b, g, n, i, slot, false) : -1;
+      s_at[tid] = page >= 0 ? page * c.page_stride + g * c.head_stride + slot * c.slot_stride : -1;
+#pragma unroll
+      for (int h = 0; h < HT; h++) {
+        uint32_t o = 0;
+        if (page >= 0 && h < hn) {
+          const uint64_t at = (row0 + h) * a.max_keys + i;
+          const int64_t sum = a.sum[row0 + h], top = ((int64_t)a.exp_out[at] << a.soft_shift) + sum / 2;
+          if (sum > 0) {
+            // the quotient is at most 2^20: a 64-bit floating point estimate is off by one at most
+            int64_t k = (int64_t)((double)top / (double)sum);
+            const int64_t r = top - k * sum;
+            k += r < 0 ? -1 : r >= sum ? 1 : 0;
+            o = (uint32_t)k;
+          }
+          if (a.softmax && part == 0) a.softmax[at] = (int32_t)o;
+        }
+        s_raw[(3 * h) * VA_STRIDE + tid] = (unsigned char)o;
+        s_raw[(3 * h + 1) * VA_STRIDE + tid] = (unsigned char)(o >> 8);
+        s_raw[(3 * h + 2) * VA_STRIDE + tid] = (unsigned char)(o >> 16);
+        uint32_t warp_sum = __reduce_add_sync(~0u, o);  // at most 32 x 2^20
+        if (lane == 0 && warp_sum) atomicAdd(&s_total[h], (unsigned long long)warp_sum);
+      }
+#pragma unroll
+      for (int k = 3 * HT; k < 8 * NT; k++) s_raw[k * VA_STRIDE + tid] = 0;
+    }
+    __syncthreads();
+    for (uint32_t k0 = wk * 32; k0 < VA_KEYS && base + k0 < last; k0 += groups * 32) {
+      uint4 v[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int64_t at = s_at[k0 + 8 * t + j];
+        v[j] = in_row && at >= 0 ? load_once(c.v + at + byte) : make_uint4(0, 0, 0, 0);
+      }
+      uint2 d[NT];
+#pragma unroll
+      for (int k = 0; k < NT; k++) d[k] = *reinterpret_cast<const uint2*>(s_raw + (k * 8 + gl) * VA_STRIDE + k0 + 8 * t);
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        uint32_t p[4], r[4];
+        auto word = [&](int j) { return w == 0 ? v[j].x : w == 1 ? v[j].y : w == 2 ? v[j].z : v[j].w; };
+        turn4(word(0), word(1), word(2), word(3), p);
+        turn4(word(4), word(5), word(6), word(7), r);
+        p[3] ^= 0x80808080u;
+        r[3] ^= 0x80808080u;
+        if (EB == 2) { p[1] ^= 0x80808080u; r[1] ^= 0x80808080u; }
+#pragma unroll
+        for (int k = 0; k < NT; k++) {
+          mma_u8u8(acc[2 * w][k], p[0], p[1], r[0], r[1], d[k].x, d[k].y);
+          mma_u8u8(acc[2 * w + 1][k], p[2], p[3], r[2], r[3], d[k].x, d[k].y);
+        }
+      }
+    }
+  }
+
+  // weights of the byte planes in the lane; digits and the warps that dealt the keys through shared memory:
+  // s_part[warp][column of eight][channel], eight columns at a time
+  int64_t* s_part = reinterpret_cast<int64_t*>(s_raw);
+  const uint32_t outputs = a.v_split * ELEMS;  // channels of the block
+  constexpr int MINE = (HT * VA_THREADS / 32 * ELEMS + VA_THREADS - 1) / VA_THREADS;  // (head, channel) of a thread at most
+  uint64_t mine[MINE];
+#pragma unroll
+  for (int i = 0; i < MINE; i++) mine[i] = 0;
+#pragma unroll
+  for (int k = 0; k < NT; k++) {
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const uint64_t a0 = (uint64_t)(int64_t)acc[2 * w][k][half] + ((uint64_t)(int64_t)acc[2 * w][k][2 + half] << 8);
+        const uint64_t a1 = (uint64_t)(int64_t)acc[2 * w + 1][k][half] + ((uint64_t)(int64_t)acc[2 * w + 1][k][2 + half] << 8);
+        int64_t* to = s_part + ((uint64_t)warp * 8 + 2 * t + half) * ELEMS;
+        if (EB == 4) {
+          to[gl * 4 + w] = (int64_t)(a0 + (a1 << 16));
+        } else {
+          to[gl * 8 + 2 * w] = (int64_t)a0;
+          to[gl * 8 + 2 * w + 1] = (int64_t)a1;
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+      const uint32_t at = i * VA_THREADS + tid, h = at / outputs, ch = at % outputs;
+      if (h < hn) {
+        for (uint32_t r = 0; r < 3; r++) {
+          const uint32_t col = 3 * h + r;
+          if (col / 8 != k) continue;
+          uint64_t v = 0;
+          for (uint32_t z = 0; z < groups; z++)
+            v += (uint64_t)s_part[((uint64_t)(z * a.v_split + ch / ELEMS) * 8 + col % 8) * ELEMS + ch % ELEMS];
+          mine[i] += v << (8 * r);
+        }
+      }
+    }
+  }
+  const uint64_t bias = EB == 4 ? uint64_t(1) << 31 : uint64_t(1) << 15;
+  const uint32_t used = (cols + a.v_chunk_keys - 1) / a.v_chunk_keys;
+  const uint32_t ch0 = part * outputs;
   bool range = false;
-  const int64_t acc = a.acc[i], y = rdiv(acc, a.soft_shift);
-  a.out[i] = saturate(y, INT32_MIN, INT32_MAX, range);
-  if (a.out_rem) a.out_rem[i] = (int32_t)(uint32_t)((uint64_t)acc - ((uint64_t)y << a.soft_shift));
-  if (range) kv_flag(a.c, STATUS_KV_RANGE);
-  if (i == row * a.c.head_dim && a.sum[row] == 0 && columns(a, (uint32_t)(row / a.heads), false)) kv_flag(a.c, STATUS_KV_EXP);
+  auto finish = [&](int64_t sum, uint64_t at) {
+    const int64_t y = rdiv(sum, a.soft_shift);
+    a.out[at] = saturate(y, INT32_MIN, INT32_MAX, range);
+    if (a.out_rem) a.out_rem[at] = (int32_t)(uint32_t)((uint64_t)sum - ((uint64_t)y << a.soft_shift));
+  };
+#pragma unroll
+  for (int i = 0; i < MINE; i++) {
+    const uint32_t at = i * VA_THREADS + tid, h = at / outputs, ch = ch0 + at % outputs;
+    if (h < hn && ch < D) {
+      const uint64_t v = mine[i] - bias * (uint64_t)s_total[h], to = (row0 + h) * D + ch;
+      if (used == 1) finish((int64_t)v, to);
+      else atomicAdd(reinterpret_cast<unsigned long long*>(a.acc + to), (unsigned long long)v);
+    }
+  }
+  if (used > 1) {
+    // the last of the row's blocks brings the sums to the output
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s_last = atomicAdd(a.done + (((uint64_t)row * a.v_tiles + tile) * a.v_parts + part), 1u) == used - 1;
+    __syncthreads();
+    if (s_last) {
+      __threadfence();
+      for (uint32_t at = tid; at < hn * outputs; at += VA_THREADS) {
+        const uint32_t h = at / outputs, ch = ch0 + at % outputs;
+        if (ch < D) finish(__ldcg(a.acc + (row0 + h) * D + ch), (row0 + h) * D + ch);
+      }
+    }
+  }
+  if (range) kv_flag(c, STATUS_KV_RANGE);
+  if (chunk == 0 && part == 0 && tid < hn && a.sum[row0 + tid] == 0) kv_flag(c, STATUS_KV_EXP);
+}
+
+template <int EB>
+static int launch_scores(grape_ctx* ctx, const AttendArgs& a, uint32_t ht, uint32_t grid, uint32_t threads, size_t smem) {
+  auto kernel = ht == 1 ? k_kv_scores<EB, 1> : ht == 2 ? k_kv_scores<EB, 2> : ht == 4 ? k_kv_scores<EB, 4> : k_kv_scores<EB, 8>;
+  GRAPE_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SC_SMEM));
+  kernel<<<grid, threads, smem, ctx->stream>>>(a);
+  return GRAPE_OK;
+}
+
+template <int EB>
+static void launch_values(grape_ctx* ctx, const AttendArgs& a, uint32_t ht, uint32_t grid) {
+  auto kernel = ht == 1 ? k_kv_values<EB, 1> : ht == 2 ? k_kv_values<EB, 2> : ht == 5 ? k_kv_values<EB, 5> : k_kv_values<EB, 8>;
+  kernel<<<grid, VA_THREADS, 0, ctx->stream>>>(a);
 }
 
 static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs& a) {
-  const uint64_t rows = (uint64_t)a.c.batch * a.heads, D = cache->head_dim;
-  a.chunk_keys = 256;
+  const uint64_t rows = (uint64_t)a.c.batch * a.heads, D = cache->head_dim, kv_rows = (uint64_t)a.c.batch * cache->kv_heads;
   const uint64_t all = a.selected ? (uint64_t)a.n_select * cache->page_size : (uint64_t)a.c.width * cache->page_size;
-  const uint64_t chunks = (std::min(all, a.max_keys) + a.chunk_keys - 1) / a.chunk_keys;
-  if (rows * chunks > 0x7fffffffu || rows * D > (uint64_t(1) << 38))
+  const uint64_t cols = std::min(all, a.max_keys);
+  const uint32_t row_bytes = (uint32_t)(D * cache->bits / 8), sms = (uint32_t)ctx->sm_count;
+
+  // Scores: heads of a block (their columns are 8 times a key's bytes), warps that share a row of long keys
+  // (eight 64-byte steps each at least), and keys of a block: 256 KB of them, fewer while that leaves the GPU
+  // with under four blocks an SM.
+  uint32_t ht = 1;
+  while (ht < 8 && ht < a.group && (uint64_t)2 * ht * row_bytes * 8 <= SC_SMEM) ht *= 2;
+  a.tiles = (a.group + ht - 1) / ht;
+  const uint32_t blks = (row_bytes + 63) / 64;
+  const size_t smem = (size_t)blks * ht * 512;
+  const uint32_t threads = smem > 64 * 1024 ? 512 : 256;
+  a.split = 1;
+  while (a.split < threads / 32 && blks / (2 * a.split) >= 8) a.split *= 2;
+  const uint32_t step = threads / 32 / a.split * 16;
+  uint64_t keys = std::max<uint64_t>(step, (256 * 1024 / row_bytes + step - 1) / step * step);
+  while (keys > step && kv_rows * a.tiles * ((cols + keys - 1) / keys) < 4ull * sms) keys = std::max<uint64_t>(step, keys / 2 / step * step);
+  a.chunk_keys = (uint32_t)keys;
+  const uint64_t chunks = (cols + keys - 1) / keys, exp_chunks = (cols + EX_KEYS - 1) / EX_KEYS;
+
+  // Values: heads of a block (three columns each, in eights), 128-byte segments of a row dealt to the warps,
+  // the rest of the warps share the keys.
+  const uint32_t v_ht = a.group == 1 ? 1 : a.group == 2 ? 2 : a.group <= 5 ? 5 : 8;
+  a.v_tiles = (a.group + v_ht - 1) / v_ht;
+  const uint32_t segments = (row_bytes + 127) / 128;
+  a.v_split = 1;
+  while (a.v_split < VA_THREADS / 32 && a.v_split < segments) a.v_split *= 2;
+  a.v_parts = (segments + a.v_split - 1) / a.v_split;
+  const uint32_t v_step = VA_THREADS / 32 / a.v_split * 32;
+  uint64_t v_keys = std::max<uint64_t>(VA_KEYS, (256 * 1024 / (a.v_split * 128) + VA_KEYS - 1) / VA_KEYS * VA_KEYS);
+  while (v_keys > v_step && kv_rows * a.v_tiles * a.v_parts * ((cols + v_keys - 1) / v_keys) < 4ull * sms)
+    v_keys = std::max<uint64_t>(v_step, v_keys / 2 / v_step * v_step);
+  a.v_chunk_keys = (uint32_t)std::min<uint64_t>(v_keys, VA_MAX_CHUNK);
+  const uint64_t v_chunks = (cols + a.v_chunk_keys - 1) / a.v_chunk_keys;
+
+  const uint64_t most = 0x7fffffffu;
+  if (kv_rows * a.tiles * chunks > most || rows * exp_chunks > most || kv_rows * a.v_tiles * a.v_parts * v_chunks > most ||
+      rows * D > (uint64_t(1) << 38))
     return kv_refuse(ctx, GRAPE_ERR_LIMIT, "too many rows and columns for one call");
   a.chunks = (uint32_t)chunks;
+  a.exp_chunks = (uint32_t)exp_chunks;
+  a.v_chunks = (uint32_t)v_chunks;
+  const uint64_t dones = kv_rows * a.v_tiles * a.v_parts;
+  a.done_per_tile = (uint32_t)((uint64_t)a.v_tiles * a.v_parts);  // zeroed by the first tile of a key head
   auto up = [](uint64_t n) { return (n + 255) & ~uint64_t(255); };
-  const uint64_t b_max = up(rows * chunks * 4), b_acc = up(rows * D * 8), b_sum = a.sum ? 0 : up(rows * 8);
+  const uint64_t b_max = up(rows * chunks * 4), b_acc = up(rows * D * 8), b_done = up(dones * 4), b_sum = a.sum ? 0 : up(rows * 8);
   const uint64_t b_keys = up(rows * a.max_keys * 4);
   void* w = nullptr;
-  if (int rc = kv_workspace(ctx, b_max + b_acc + b_sum + (a.score ? 0 : b_keys) + (a.exp_out ? 0 : b_keys), &w)) return rc;
+  if (int rc = kv_workspace(ctx, b_max + b_acc + b_done + b_sum + (a.score ? 0 : b_keys) + (a.exp_out ? 0 : b_keys), &w)) return rc;
   char* p = reinterpret_cast<char*>(w);
   a.chunk_max = reinterpret_cast<int32_t*>(p);
   p += b_max;
   a.acc = reinterpret_cast<int64_t*>(p);
   p += b_acc;
+  a.done = reinterpret_cast<uint32_t*>(p);
+  p += b_done;
   if (!a.sum) { a.sum = reinterpret_cast<int64_t*>(p); p += b_sum; }
   if (!a.score) { a.score = reinterpret_cast<int32_t*>(p); p += b_keys; }
   if (!a.exp_out) { a.exp_out = reinterpret_cast<int32_t*>(p); p += b_keys; }
-  const uint32_t grid = (uint32_t)(rows * chunks);
-  if (cache->bits == 32) k_kv_scores<4><<<grid, AT_THREADS, 0, ctx->stream>>>(a);
-  else k_kv_scores<2><<<grid, AT_THREADS, 0, ctx->stream>>>(a);
-  k_kv_exp<<<grid, AT_THREADS, 0, ctx->stream>>>(a);
-  if (cache->bits == 32) k_kv_values<4><<<grid, AT_THREADS, 0, ctx->stream>>>(a);
-  else k_kv_values<2><<<grid, AT_THREADS, 0, ctx->stream>>>(a);
-  k_kv_out<<<(uint32_t)((rows * D + AT_THREADS - 1) / AT_THREADS), AT_THREADS, 0, ctx->stream>>>(a, rows * D);
-  ctx->launches += 4;
+
+  const uint32_t grid = (uint32_t)(kv_rows * a.tiles * chunks), v_grid = (uint32_t)(dones * v_chunks);
+  if (int rc = cache->bits == 32 ? launch_scores<4>(ctx, a, ht, grid, threads, smem) : launch_scores<2>(ctx, a, ht, grid, threads, smem)) return rc;
+  if (cache->page_size % 4 == 0 && a.max_keys % 4 == 0) k_kv_exp<4><<<(uint32_t)(rows * exp_chunks), EX_THREADS, 0, ctx->stream>>>(a);
+  else k_kv_exp<1><<<(uint32_t)(rows * exp_chunks), EX_THREADS, 0, ctx->stream>>>(a);
+  if (cache->bits == 32) launch_values<4>(ctx, a, v_ht, v_grid);
+  else launch_values<2>(ctx, a, v_ht, v_grid);
+  ctx->launches += 3;
   GRAPE_CUDA_TRY(ctx, cudaGetLastError());
   return GRAPE_OK;
 }
