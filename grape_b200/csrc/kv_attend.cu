@@ -29,7 +29,9 @@ struct AttendArgs {
   uint32_t tiles, split, chunks, chunk_keys;  // scores: head tiles of a key head, warps of a row, blocks of a row
   uint32_t exp_chunks;
   uint32_t v_tiles, v_parts, v_split, v_chunks, v_chunk_keys;  // values: head tiles, parts of a row, warps of a part, ...
-  uint32_t done_per_tile;
+  uint32_t done_per_row;
+  unsigned char* valid;   // [batch][kv_heads][columns]: 1 where a column holds a position
+  uint64_t valid_stride;
 };
 
 // Columns of a row that can hold a position: its length, or the slots of the selected pages.
@@ -62,12 +64,15 @@ __device__ __forceinline__ int32_t column_page(const AttendArgs& a, uint32_t b, 
   return page;
 }
 
-// 16 bytes that are read once: past L1.
-__device__ __forceinline__ uint4 load_once(const char* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+// A lane's own queue in shared memory: 16-byte copies from global memory that this lane alone reads back, so
+// that no barrier is needed, only the wait for its own copies, and what is under way costs no registers.
+__device__ __forceinline__ void copy_async(uint4* to, const char* from, bool there) {
+  // nothing is read where `there` is false: the 16 bytes become zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void mma_u8s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -95,7 +100,8 @@ __device__ __forceinline__ void mma_u8u8(int32_t (&c)[4], uint32_t a0, uint32_t 
 // What bounds it: bytes of the keys.  The instruction takes 2 cycles of an SM (measured, 570 T products/s) for
 // 512 bytes of keys and a head, which arrive every 22 cycles.
 constexpr int SC_MAX_THREADS = 512;
-constexpr int SC_SMEM = 128 * 1024;  // columns of a block at most
+constexpr int SC_SMEM = 128 * 1024;      // bytes of a block's columns at most
+constexpr int SC_SMEM_ALL = 224 * 1024;  // and of all that it keeps in shared memory
 
 template <int EB>
 __device__ __forceinline__ uint32_t column_word(const uint64_t (&u)[4 / EB], int c) {
@@ -116,12 +122,19 @@ __device__ __forceinline__ uint32_t column_word(const uint64_t (&u)[4 / EB], int
   return w;
 }
 
+__host__ __device__ constexpr int sc_sixteens(int ht) { return ht >= 4 ? 2 : 1; }  // sixteens of keys that share a read of the columns
+__host__ __device__ constexpr int sc_stages(int ht) { return ht >= 4 ? 4 : 5; }    // steps in a lane's queue
+
 template <int EB, int HT>
 __global__ void __launch_bounds__(SC_MAX_THREADS) k_kv_scores(AttendArgs a) {
-  extern __shared__ uint4 s_w[];  // [blk][HT][32 lanes]: 4 words, the columns of a lane's 16 bytes
-  __shared__ int64_t s_part[SC_MAX_THREADS / 32 * 16 * (HT > 4 ? 4 : HT)];
+  constexpr int MT = sc_sixteens(HT), STAGES = sc_stages(HT);
+  constexpr int NV = 2 * MT * HT;               // values of a lane group: (head, eight of keys)
+  constexpr int OWN = NV >= 4 ? NV / 4 : 1;     // those that a lane finishes
+  constexpr int HEADS = HT >= 4 ? HT / 4 : 1;   // and the heads they belong to
+  extern __shared__ uint4 s_w[];  // [blk][HT][32 lanes]: 4 words, the columns of a lane's 16 bytes; the lanes' queues; partial sums
   __shared__ unsigned long long s_bias[HT];
   __shared__ int32_t s_max[HT];
+  __shared__ unsigned char s_valid[SC_MAX_THREADS / 32][16 * MT];
   const KvView& c = a.c;
   const uint32_t D = c.head_dim, row_bytes = D * EB, blks = (row_bytes + 63) / 64;
   uint32_t x = blockIdx.x;
@@ -137,7 +150,7 @@ __global__ void __launch_bounds__(SC_MAX_THREADS) k_kv_scores(AttendArgs a) {
     // what the later passes add to
     for (uint32_t i = tid; i < hn * D; i += blockDim.x) a.acc[row0 * D + i] = 0;
     for (uint32_t i = tid; i < hn; i += blockDim.x) a.sum[row0 + i] = 0;
-    for (uint32_t i = tid; tile == 0 && i < a.done_per_tile; i += blockDim.x) a.done[(uint64_t)row * a.done_per_tile + i] = 0;
+    for (uint32_t i = tid; tile == 0 && i < a.done_per_row; i += blockDim.x) a.done[(uint64_t)row * a.done_per_row + i] = 0;
     if (cols == 0) {
       for (uint32_t i = tid; i < hn * D; i += blockDim.x) {
         a.out[row0 * D + i] = 0;
@@ -148,18 +161,60 @@ __global__ void __launch_bounds__(SC_MAX_THREADS) k_kv_scores(AttendArgs a) {
   const uint32_t first = chunk * a.chunk_keys, last = min(cols, first + a.chunk_keys);
   if (first >= last) return;
 
+  const uint32_t gl = lane >> 2, t = lane & 3;
+  const uint32_t wd = warp % a.split, wk = warp / a.split, keys_at_once = warps / a.split * 16 * MT;
+  const uint32_t blk0 = blks * wd / a.split, blk1 = blks * (wd + 1) / a.split;
+
+  // A step is 64 bytes of the warp's 16 MT keys.  `fetch` walks the steps STAGES - 1 ahead of their use; which of
+  // a lane's keys exist goes through `fifo`, four bits for each set of keys under way.
+  uint4* const queue = s_w + (uint64_t)blks * HT * 32 + (uint64_t)warp * STAGES * MT * 64 + lane;
+  const char* key[2 * MT];
+  uint32_t ahead_base = first, ahead_blk = blk0, ahead_slot = 0, fifo = 0, under_way = 0;
+  auto fetch = [&]() {
+    if (ahead_base < last) {
+      if (ahead_blk == blk0) {
+        uint32_t mask = 0;
+#pragma unroll
+        for (int m = 0; m < 2 * MT; m++) {
+          const uint32_t i = ahead_base + wk * 16 * MT + m * 8 + gl;
+          uint32_t slot;
+          const int32_t page = i < last ? column_page(a, b, g, n, i, slot, t == 0 && wd == 0) : -1;
+          key[m] = page >= 0 ? c.k + page * c.page_stride + g * c.head_stride + slot * c.slot_stride + t * 16 : nullptr;
+          if (page >= 0) mask |= 1u << m;
+        }
+        fifo |= mask << (4 * under_way++);
+      }
+      const bool in = ahead_blk * 64 + t * 16 < row_bytes;
+#pragma unroll
+      for (int m = 0; m < 2 * MT; m++) {
+        const bool there = in && key[m];
+        copy_async(queue + (ahead_slot * 2 * MT + m) * 32, there ? key[m] + ahead_blk * 64 : c.k, there);
+      }
+      ahead_slot = ahead_slot + 1 == STAGES ? 0 : ahead_slot + 1;
+      if (++ahead_blk == blk1) {
+        ahead_blk = blk0;
+        ahead_base += keys_at_once;
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll 1
+  for (int i = 0; i < STAGES - 1; i++) fetch();
+
+  // the operand columns, and the sum of each head's query
   if (tid < HT) { s_bias[tid] = 0; s_max[tid] = INT32_MIN; }
   __syncthreads();
-  const int32_t* q = a.q + (uint64_t)b * a.q_stride + (uint64_t)h0 * D;
-  constexpr uint32_t PER = 4 / EB;  // elements of a word
-  for (uint32_t h = 0; h < HT; h++) {
+  {
+    constexpr uint32_t PER = 4 / EB;  // elements of a word
+    const uint32_t share = blockDim.x / HT, h = tid / share;
+    const int32_t* q = a.q + (uint64_t)b * a.q_stride + (uint64_t)(h0 + h) * D;
     int64_t total = 0;
-    for (uint32_t i = tid; i < blks * 16; i += blockDim.x) {
+    for (uint32_t i = tid % share; i < blks * 16; i += share) {
       uint64_t u[PER];
 #pragma unroll
       for (uint32_t e = 0; e < PER; e++) {
         const uint32_t d = i * PER + e;
-        const int32_t v = h < hn && d < D ? __ldg(q + (uint64_t)h * D + d) : 0;
+        const int32_t v = h < hn && d < D ? __ldg(q + d) : 0;
         total += v;
         u[e] = (uint64_t)((int64_t)v + 0x80808080ll);
       }
@@ -173,14 +228,11 @@ __global__ void __launch_bounds__(SC_MAX_THREADS) k_kv_scores(AttendArgs a) {
   }
   __syncthreads();
 
-  const uint32_t gl = lane >> 2, t = lane & 3;
-  const uint32_t wd = warp % a.split, wk = warp / a.split, keys_at_once = warps / a.split * 16;
-  const uint32_t blk0 = blks * wd / a.split, blk1 = blks * (wd + 1) / a.split;
   const uint64_t bias = EB == 4 ? uint64_t(1) << 31 : uint64_t(1) << 15;
   constexpr uint32_t FLIP = EB == 4 ? 0x80000000u : 0x80008000u;
-  int32_t best[HT];
+  int32_t best[HEADS];
 #pragma unroll
-  for (int h = 0; h < HT; h++) best[h] = INT32_MIN;
+  for (int j = 0; j < HEADS; j++) best[j] = INT32_MIN;
   bool range = false;
   auto finish = [&](uint64_t acc, uint32_t h, uint32_t i) {
     acc -= bias * (uint64_t)s_bias[h];
@@ -192,161 +244,154 @@ __global__ void __launch_bounds__(SC_MAX_THREADS) k_kv_scores(AttendArgs a) {
     return v;
   };
 
+  uint32_t slot = 0;
   for (uint32_t base = first; base < last; base += keys_at_once) {
-    const uint32_t i0 = base + wk * 16 + gl, i1 = i0 + 8;
-    const char* k0 = nullptr;
-    const char* k1 = nullptr;
-    uint32_t slot;
-    if (i0 < last) {
-      const int32_t page = column_page(a, b, g, n, i0, slot, t == 0 && wd == 0);
-      if (page >= 0) k0 = c.k + page * c.page_stride + g * c.head_stride + slot * c.slot_stride + t * 16;
-    }
-    if (i1 < last) {
-      const int32_t page = column_page(a, b, g, n, i1, slot, t == 0 && wd == 0);
-      if (page >= 0) k1 = c.k + page * c.page_stride + g * c.head_stride + slot * c.slot_stride + t * 16;
-    }
-    int32_t acc[HT][4];
+    int32_t acc[HT][MT][4];
 #pragma unroll
-    for (int h = 0; h < HT; h++) acc[h][0] = acc[h][1] = acc[h][2] = acc[h][3] = 0;
-    constexpr int U = 4;
-    for (uint32_t blk = blk0; blk < blk1; blk += U) {
-      uint4 x0[U], x1[U];
+    for (int h = 0; h < HT; h++)
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const bool in = blk + u < blk1 && (blk + u) * 64 + t * 16 < row_bytes;
-        x0[u] = in && k0 ? load_once(k0 + (blk + u) * 64) : make_uint4(0, 0, 0, 0);
-        x1[u] = in && k1 ? load_once(k1 + (blk + u) * 64) : make_uint4(0, 0, 0, 0);
+      for (int m = 0; m < MT; m++) acc[h][m][0] = acc[h][m][1] = acc[h][m][2] = acc[h][m][3] = 0;
+#pragma unroll 1
+    for (uint32_t blk = blk0; blk < blk1; blk++) {
+      copy_wait<STAGES - 2>();
+      uint4 y[2 * MT];
+#pragma unroll
+      for (int m = 0; m < 2 * MT; m++) {
+        y[m] = queue[(slot * 2 * MT + m) * 32];
+        y[m].x ^= FLIP;
+        y[m].y ^= FLIP;
+        y[m].z ^= FLIP;
+        y[m].w ^= FLIP;
       }
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+      fetch();  // into the place that was read a step ago
+      const uint4* w = s_w + (uint64_t)blk * HT * 32 + lane;
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        if (blk + u >= blk1) break;
-        const uint4 y0 = make_uint4(x0[u].x ^ FLIP, x0[u].y ^ FLIP, x0[u].z ^ FLIP, x0[u].w ^ FLIP);
-        const uint4 y1 = make_uint4(x1[u].x ^ FLIP, x1[u].y ^ FLIP, x1[u].z ^ FLIP, x1[u].w ^ FLIP);
-        const uint4* w = s_w + (uint64_t)(blk + u) * HT * 32 + lane;
+      for (int h = 0; h < HT; h++) {
+        if (HT > 2 && h >= hn) break;
+        const uint4 z = w[h * 32];
 #pragma unroll
-        for (int h = 0; h < HT; h++) {
-          if (HT > 2 && h >= hn) break;
-          const uint4 m = w[h * 32];
-          mma_u8s8(acc[h], y0.x, y1.x, y0.y, y1.y, m.x, m.y);
-          mma_u8s8(acc[h], y0.z, y1.z, y0.w, y1.w, m.z, m.w);
+        for (int m = 0; m < MT; m++) {
+          mma_u8s8(acc[h][m], y[2 * m].x, y[2 * m + 1].x, y[2 * m].y, y[2 * m + 1].y, z.x, z.y);
+          mma_u8s8(acc[h][m], y[2 * m].z, y[2 * m + 1].z, y[2 * m].w, y[2 * m + 1].w, z.z, z.w);
         }
       }
     }
-    // lane (g, t) holds columns 2t and 2t + 1 of keys g and g + 8
+    const uint32_t mask = fifo & 15;
+    fifo >>= 4;
+    under_way--;
+    // Lane (g, t) holds columns 2t and 2t + 1 of keys g and g + 8.  The sum over t leaves lane t with the values
+    // t OWN .. of (head * MT + sixteen) * 2 + eight: each lane finishes its own.
+    uint64_t v[NV];
 #pragma unroll
-    for (int h = 0; h < HT; h++) {
-      uint64_t v0 = ((uint64_t)(int64_t)acc[h][0] + ((uint64_t)(int64_t)acc[h][1] << 8)) << (16 * t);
-      uint64_t v1 = ((uint64_t)(int64_t)acc[h][2] + ((uint64_t)(int64_t)acc[h][3] << 8)) << (16 * t);
-      v0 += __shfl_xor_sync(~0u, v0, 1);
-      v1 += __shfl_xor_sync(~0u, v1, 1);
-      v0 += __shfl_xor_sync(~0u, v0, 2);
-      v1 += __shfl_xor_sync(~0u, v1, 2);
-      if (a.split == 1) {
-        if (t == (h & 3) && h < hn) {
-          if (k0) best[h] = max(best[h], finish(v0, h, i0));
-          if (k1) best[h] = max(best[h], finish(v1, h, i1));
-        }
-      } else {
-        // the warps that share the keys: four heads at a time through shared memory
-        constexpr int AT_ONCE = HT > 4 ? 4 : HT;
-        if (h % AT_ONCE == 0) __syncthreads();
-        if (t == 0) {
-          s_part[(warp * AT_ONCE + h % AT_ONCE) * 16 + gl] = (int64_t)v0;
-          s_part[(warp * AT_ONCE + h % AT_ONCE) * 16 + gl + 8] = (int64_t)v1;
-        }
-        if (h % AT_ONCE == AT_ONCE - 1) {
-          __syncthreads();
-          // warp wd of a group adds the heads wd, wd + split, ...: lanes 0..15 the group's 16 keys, whose validity
-          // lane (gl, t) knows for keys gl and gl + 8
-          const uint32_t valid = __ballot_sync(~0u, k0 != nullptr && t == 0), valid1 = __ballot_sync(~0u, k1 != nullptr && t == 0);
+    for (int h = 0; h < HT; h++)
 #pragma unroll
-          for (int j = 0; j < AT_ONCE; j++) {
-            const int hh = h - (AT_ONCE - 1) + j;
-            if (j % a.split == wd && hh < hn && lane < 16) {
-              const bool ok = ((lane < 8 ? valid : valid1) >> ((lane & 7) * 4)) & 1;
-              uint64_t v = 0;
-              for (uint32_t w2 = 0; w2 < a.split; w2++) v += (uint64_t)s_part[((wk * a.split + w2) * AT_ONCE + j) * 16 + lane];
-              if (ok) best[hh] = max(best[hh], finish(v, hh, base + wk * 16 + lane));
-            }
-          }
-        }
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+          v[(h * MT + m) * 2 + e] = ((uint64_t)(int64_t)acc[h][m][2 * e] + ((uint64_t)(int64_t)acc[h][m][2 * e + 1] << 8)) << (16 * t);
+    if (NV >= 4) {
+#pragma unroll
+      for (int j = 0; j < NV / 2; j++) {
+        const uint64_t keep = t & 2 ? v[j + NV / 2] : v[j], give = t & 2 ? v[j] : v[j + NV / 2];
+        v[j] = keep + __shfl_xor_sync(~0u, give, 2);
+      }
+    } else {
+      v[0] += __shfl_xor_sync(~0u, v[0], 2);
+      v[1] += __shfl_xor_sync(~0u, v[1], 2);
+    }
+#pragma unroll
+    for (int j = 0; j < OWN; j++) {
+      const uint64_t keep = t & 1 ? v[j + OWN] : v[j], give = t & 1 ? v[j] : v[j + OWN];
+      v[j] = keep + __shfl_xor_sync(~0u, give, 1);
+    }
+    const uint32_t own0 = NV >= 4 ? t * OWN : t & 1, key0 = base + wk * 16 * MT + gl;
+    if (tile == 0 && wd == 0 && t < 2 * MT && key0 + t * 8 < last) a.valid[(uint64_t)row * a.valid_stride + key0 + t * 8] = (mask >> t) & 1;
+    if (a.split == 1) {
+#pragma unroll
+      for (int j = 0; j < OWN; j++) {
+        const uint32_t own = own0 + j, h = own / (2 * MT), e = own % (2 * MT);
+        if (h < hn && (NV >= 4 || t < 2) && ((mask >> e) & 1)) best[j * HEADS / OWN] = max(best[j * HEADS / OWN], finish(v[j], h, key0 + e * 8));
+      }
+    } else {
+      // warps that share the keys add up in shared memory, [warp][value][g]
+      int64_t* s_part = reinterpret_cast<int64_t*>(s_w + (uint64_t)blks * HT * 32 + (uint64_t)warps * STAGES * MT * 64);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < OWN; j++)
+        if (NV >= 4 || t < 2) s_part[((uint64_t)warp * NV + own0 + j) * 8 + gl] = (int64_t)v[j];
+      if (wd == 0 && t < 2 * MT) s_valid[wk][t * 8 + gl] = (mask >> t) & 1;
+      __syncthreads();
+      for (uint32_t i = wd * 32 + lane; i < NV * 8; i += a.split * 32) {
+        const uint32_t own = i / 8, h = own / (2 * MT), at = own % (2 * MT) * 8 + i % 8;
+        if (h >= hn || !s_valid[wk][at]) continue;
+        uint64_t sum = 0;
+        for (uint32_t w = 0; w < a.split; w++) sum += (uint64_t)s_part[((uint64_t)(wk * a.split + w) * NV + own) * 8 + i % 8];
+        atomicMax(&s_max[h], finish(sum, h, base + wk * 16 * MT + at));
       }
     }
   }
   if (range) kv_flag(c, STATUS_KV_RANGE);
+  if (a.split == 1) {
 #pragma unroll
-  for (int h = 0; h < HT; h++) {
-    for (int o = 16; o; o >>= 1) best[h] = max(best[h], __shfl_xor_sync(~0u, best[h], o));
-    if (lane == 0) atomicMax(&s_max[h], best[h]);
+    for (int j = 0; j < HEADS; j++) {
+      for (int o = 16; o >= 4; o >>= 1) best[j] = max(best[j], __shfl_xor_sync(~0u, best[j], o));
+      const uint32_t h = HT >= 4 ? t * HEADS + j : HT == 2 ? t >> 1 : 0;
+      if (gl == 0) atomicMax(&s_max[h], best[j]);
+    }
   }
   __syncthreads();
   if (tid < hn) a.chunk_max[(row0 + tid) * a.chunks + chunk] = s_max[tid];
 }
 
 // ---- exp -----------------------------------------------------------------------------------------
-// exp_in, exp_out and the row's sum; V columns of a row per thread (4 where they share a page and 16 bytes).
-constexpr int EX_THREADS = 256;
-constexpr uint32_t EX_KEYS = 2048;  // columns of a block
+// exp_in, exp_out and the row's sum.  The table (4 MB for the layer prover's) lives in L2; a thread has four
+// columns under way, since what it waits for is a chain of three loads.
+constexpr int EX_THREADS = 256, EX_COLS = 4;
+constexpr uint32_t EX_KEYS = EX_THREADS * EX_COLS;  // columns of a block
 
-template <int V>
 __global__ void __launch_bounds__(EX_THREADS) k_kv_exp(AttendArgs a) {
   __shared__ int32_t s_max[EX_THREADS / 32];
   __shared__ int64_t s_sum[EX_THREADS / 32];
   const KvView& c = a.c;
   const uint32_t chunk = blockIdx.x % a.exp_chunks, row = blockIdx.x / a.exp_chunks, h = row % a.heads, b = row / a.heads, g = h / a.group;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t n = kv_length(c, a.len, b, a.selected ? ~0ull : a.max_keys, false), cols = columns(a, b, false);
-  const uint32_t first = chunk * EX_KEYS, last = min(cols, first + EX_KEYS);
-  if (first >= last) return;
+  const uint32_t cols = columns(a, b, false), first = chunk * EX_KEYS + threadIdx.x;
+  if (chunk * EX_KEYS >= cols) return;
+  const uint64_t at = (uint64_t)row * a.max_keys + first;
+  const unsigned char* valid = a.valid + ((uint64_t)b * c.kv_heads + g) * a.valid_stride + first;
+  bool in[EX_COLS];
+  int32_t s[EX_COLS];
+#pragma unroll
+  for (int j = 0; j < EX_COLS; j++) {
+    in[j] = first + j * EX_THREADS < cols && valid[j * EX_THREADS];
+    s[j] = first + j * EX_THREADS < cols ? a.score[at + j * EX_THREADS] : 0;
+  }
   int32_t best = INT32_MIN;
   const uint32_t used = (cols + a.chunk_keys - 1) / a.chunk_keys;
   for (uint32_t i = threadIdx.x; i < used; i += EX_THREADS) best = max(best, a.chunk_max[(uint64_t)row * a.chunks + i]);
-  for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
+  best = __reduce_max_sync(~0u, best);
   if (lane == 0) s_max[warp] = best;
   __syncthreads();
+#pragma unroll
   for (int w = 0; w < EX_THREADS / 32; w++) best = max(best, s_max[w]);
-  const int64_t top = best;
   int64_t sum = 0;
   bool outside = false;
-  for (uint32_t i = first + threadIdx.x * V; i < last; i += EX_THREADS * V) {
-    uint32_t slot;
-    if (column_page(a, b, g, n, i, slot, false) < 0) continue;
-    const uint64_t at = (uint64_t)row * a.max_keys + i;
-    // how many of the V columns hold a position: the page's last tokens may end inside
-    uint32_t m = V;
-    if (V > 1) {
-      m = min(m, last - i);
-      for (uint32_t j = 1; j < m; j++)
-        if (column_page(a, b, g, n, i + j, slot, false) < 0) { m = j; break; }
-    }
-    int32_t s[V], x[V], e[V];
-    if (V == 4 && m == 4) {
-      const int4 v = *reinterpret_cast<const int4*>(a.score + at);
-      s[0] = v.x; s[1 % V] = v.y; s[2 % V] = v.z; s[3 % V] = v.w;
-    } else {
-      for (uint32_t j = 0; j < V; j++) s[j] = j < m ? a.score[at + j] : (int32_t)top;
-    }
+  int32_t x[EX_COLS], e[EX_COLS];
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-      const int64_t d = s[j] - top;
-      if (d < a.exp_low) outside = true;
-      x[j] = (int32_t)max(d, (int64_t)a.exp_low);
-      e[j] = __ldg(a.exp + (x[j] - a.exp_low));
-    }
+  for (int j = 0; j < EX_COLS; j++) {
+    const int64_t d = in[j] ? (int64_t)s[j] - best : 0;
+    outside |= d < a.exp_low;
+    x[j] = (int32_t)max(d, (int64_t)a.exp_low);
+    e[j] = __ldg(a.exp + (x[j] - a.exp_low));
+  }
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-      if (e[j] < 0) { e[j] = 0; outside = true; }
-      if (j < m) sum += e[j];
-    }
-    if (V == 4 && m == 4) {
-      if (a.exp_in) *reinterpret_cast<int4*>(a.exp_in + at) = make_int4(x[0], x[1 % V], x[2 % V], x[3 % V]);
-      *reinterpret_cast<int4*>(a.exp_out + at) = make_int4(e[0], e[1 % V], e[2 % V], e[3 % V]);
-    } else {
-      for (uint32_t j = 0; j < m; j++) {
-        if (a.exp_in) a.exp_in[at + j] = x[j];
-        a.exp_out[at + j] = e[j];
-      }
-    }
+  for (int j = 0; j < EX_COLS; j++) {
+    if (!in[j]) continue;
+    if (e[j] < 0) { e[j] = 0; outside = true; }
+    sum += e[j];
+    if (a.exp_in) a.exp_in[at + j * EX_THREADS] = x[j];
+    a.exp_out[at + j * EX_THREADS] = e[j];
   }
   if (outside) kv_flag(c, STATUS_KV_EXP);
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
@@ -364,11 +409,18 @@ __global__ void __launch_bounds__(EX_THREADS) k_kv_exp(AttendArgs a) {
 //   sum_j o_j v_j = sum_p,r 256^(p + r) (byte plane p of v' . digit r of o) - bias sum_j o_j.
 // A warp takes 32 keys x 128 bytes of their rows: lane (g, t) loads 16 bytes of the 8 keys 8t .. 8t+7, and
 // turning 4 keys x 4 bytes in registers (8 byte permutes) gives the A registers, keys along the instruction's
-// inner dimension.  Sums of a chunk of at most 16384 keys stay below 16384 x 255 x 255 < 2^31.
-constexpr int VA_THREADS = 256;
-constexpr uint32_t VA_KEYS = 256;          // keys whose softmax a block holds at a time
-constexpr uint32_t VA_STRIDE = VA_KEYS + 32;  // of a column's digits: eight columns on different banks
-constexpr uint32_t VA_MAX_CHUNK = 16384;
+// inner dimension.  Sums of a chunk of at most 1024 keys stay far below 2^31.  The 8 bytes of digits that a lane
+// needs for 32 keys lie together in shared memory.
+// What bounds it: bytes of the values; 32 keys x 128 bytes cost a warp about 100 instructions of the 700 that
+// an SM quarter issues while they arrive.
+constexpr uint32_t VA_CHUNK = 1024;           // keys of a block at most
+constexpr uint32_t VA_STRIDE = VA_CHUNK + 32; // bytes of a column's digits: eight columns on different banks
+__host__ __device__ constexpr int va_tiles(int ht) { return (3 * ht + 7) / 8; }                   // instruction columns in eights
+__host__ __device__ constexpr int va_threads(int ht) { return va_tiles(ht) > 2 ? 128 : 256; }     // by the registers of the sums
+constexpr int VA_STAGES = 2;
+constexpr size_t va_smem(int ht) {  // queues (later partial sums of 8 columns), digits, places of the keys
+  return (size_t)va_threads(ht) / 32 * VA_STAGES * 4096 + (size_t)VA_STRIDE * 8 * va_tiles(ht) + VA_CHUNK * 8;
+}
 
 // bytes [key][plane] of 4 words -> words [plane] of 4 keys
 __device__ __forceinline__ void turn4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&o)[4]) {
@@ -381,14 +433,16 @@ __device__ __forceinline__ void turn4(uint32_t a, uint32_t b, uint32_t c, uint32
 }
 
 template <int EB, int HT>
-__global__ void __launch_bounds__(VA_THREADS) k_kv_values(AttendArgs a) {
-  constexpr int NT = (3 * HT + 7) / 8;       // instruction columns in eights
+__global__ void __launch_bounds__(va_threads(HT), 512 / va_threads(HT) - (va_tiles(HT) > 2 ? 1 : 0)) k_kv_values(AttendArgs a) {
+  constexpr int NT = va_tiles(HT), THREADS = va_threads(HT);
   constexpr uint32_t ELEMS = 128 / EB;       // channels of a warp
-  constexpr uint32_t DIGITS = VA_STRIDE * 8 * NT, PART = VA_THREADS / 32 * 8 * ELEMS * 8;
-  __shared__ __align__(16) unsigned char s_raw[DIGITS > PART ? DIGITS : PART];  // digits [column][key], later partial sums
-  __shared__ __align__(16) int64_t s_at[VA_KEYS];
+  extern __shared__ uint4 s_dyn[];
   __shared__ unsigned long long s_total[HT];
+  __shared__ int64_t s_sum[HT];
+  __shared__ double s_inverse[HT];
   __shared__ uint32_t s_last;
+  unsigned char* const s_digits = reinterpret_cast<unsigned char*>(s_dyn + THREADS / 32 * VA_STAGES * 256);
+  int64_t* const s_at = reinterpret_cast<int64_t*>(s_digits + VA_STRIDE * 8 * NT);
   const KvView& c = a.c;
   const uint32_t D = c.head_dim, row_bytes = D * EB, segments = (row_bytes + 127) / 128;
   uint32_t x = blockIdx.x;
@@ -400,86 +454,111 @@ __global__ void __launch_bounds__(VA_THREADS) k_kv_values(AttendArgs a) {
   const uint32_t h0 = g * a.group + tile * HT, hn = min((uint32_t)HT, a.group - tile * HT);
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t = lane & 3;
   const uint32_t n = kv_length(c, a.len, b, a.selected ? ~0ull : a.max_keys, false), cols = columns(a, b, false);
-  const uint32_t first = chunk * a.v_chunk_keys, last = min(cols, first + a.v_chunk_keys);
-  if (first >= last) return;
+  const uint32_t first = chunk * a.v_chunk_keys, keys = min(cols, first + a.v_chunk_keys) - first;
+  if (first >= cols) return;
   const uint64_t row0 = (uint64_t)b * a.heads + h0;
-  const uint32_t wd = warp % a.v_split, wk = warp / a.v_split, groups = VA_THREADS / 32 / a.v_split;
+  const uint32_t wd = warp % a.v_split, wk = warp / a.v_split, groups = THREADS / 32 / a.v_split;
   const uint32_t segment = part * a.v_split + wd, byte = segment * 128 + gl * 16;
   const bool in_row = segment < segments && byte < row_bytes;
-  if (tid < HT) s_total[tid] = 0;
+  const uint32_t padded = (keys + 31) & ~31u;
+  for (uint32_t j = tid; j < padded; j += THREADS) {
+    uint32_t slot = 0;
+    const int32_t page = j < keys ? column_page(a, b, g, n, first + j, slot, false) : -1;
+    s_at[j] = page >= 0 ? page * c.page_stride + g * c.head_stride + slot * c.slot_stride : -1;
+  }
+  if (tid < HT) {
+    s_total[tid] = 0;
+    s_sum[tid] = tid < hn ? a.sum[row0 + tid] : 0;
+    s_inverse[tid] = s_sum[tid] > 0 ? 1.0 / (double)s_sum[tid] : 0.0;
+  }
+  __syncthreads();
+
+  uint4* const queue = s_dyn + (uint64_t)warp * VA_STAGES * 256 + lane;
+  auto fetch = [&](uint32_t k0, uint32_t stage) {
+    if (k0 < padded) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int64_t at = s_at[k0 + 8 * t + j];
+        const bool there = in_row && at >= 0;
+        copy_async(queue + (stage * 8 + j) * 32, there ? c.v + at + byte : c.v, there);
+      }
+    }
+    copy_commit();
+  };
+  fetch(wk * 32, 0);
+  fetch((wk + groups) * 32, 1);
+
+  // the softmax of the chunk, while the first values are under way
+  for (uint32_t j = tid; j < padded; j += THREADS) {
+    const bool there = s_at[j] >= 0;
+    int32_t e[HT];
+#pragma unroll
+    for (int h = 0; h < HT; h++) e[h] = there && h < hn ? a.exp_out[(row0 + h) * a.max_keys + first + j] : 0;
+#pragma unroll
+    for (int h = 0; h < HT; h++) {
+      uint32_t o = 0;
+      if (there && h < hn) {
+        const int64_t sum = s_sum[h], top = ((int64_t)e[h] << a.soft_shift) + sum / 2;
+        if (sum > 0) {
+          // the quotient is at most 2^20: a 64-bit floating point estimate is off by one at most
+          int64_t k = (int64_t)((double)top * s_inverse[h]);
+          const int64_t r = top - k * sum;
+          k += r < 0 ? -1 : r >= sum ? 1 : 0;
+          o = (uint32_t)k;
+        }
+        if (a.softmax && part == 0) a.softmax[(row0 + h) * a.max_keys + first + j] = (int32_t)o;
+      }
+      s_digits[(3 * h) * VA_STRIDE + j] = (unsigned char)o;
+      s_digits[(3 * h + 1) * VA_STRIDE + j] = (unsigned char)(o >> 8);
+      s_digits[(3 * h + 2) * VA_STRIDE + j] = (unsigned char)(o >> 16);
+      const uint32_t warp_sum = __reduce_add_sync(~0u, o);  // at most 32 x 2^20; whole warps: padded is a multiple of 32
+      if (lane == 0 && warp_sum) atomicAdd(&s_total[h], (unsigned long long)warp_sum);
+    }
+#pragma unroll
+    for (int k = 3 * HT; k < 8 * NT; k++) s_digits[k * VA_STRIDE + j] = 0;
+  }
+  __syncthreads();
+
   int32_t acc[8][NT][4];
 #pragma unroll
   for (int m = 0; m < 8; m++)
 #pragma unroll
     for (int k = 0; k < NT; k++) acc[m][k][0] = acc[m][k][1] = acc[m][k][2] = acc[m][k][3] = 0;
-
-  for (uint32_t base = first; base < last; base += VA_KEYS) {
-    __syncthreads();
-    // the softmax of the next keys, a thread a key
-    {
-      static_assert(VA_KEYS == VA_THREADS, "a thread a key");
-      const uint32_t i = base + tid;
-      uint32_t slot = 0;
-      const int32_t page = i < last ? column_page(a, b, g, n, i, slot, false) : -1;
-      s_at[tid] = page >= 0 ? page * c.page_stride + g * c.head_stride + slot * c.slot_stride : -1;
+  uint32_t stage = 0;
+#pragma unroll 1
+  for (uint32_t k0 = wk * 32; k0 < padded; k0 += groups * 32) {
+    copy_wait<VA_STAGES - 1>();
+    uint4 v[8];
 #pragma unroll
-      for (int h = 0; h < HT; h++) {
-        uint32_t o = 0;
-        if (page >= 0 && h < hn) {
-          const uint64_t at = (row0 + h) * a.max_keys + i;
-          const int64_t sum = a.sum[row0 + h], top = ((int64_t)a.exp_out[at] << a.soft_shift) + sum / 2;
-          if (sum > 0) {
-            // the quotient is at most 2^20: a 64-bit floating point estimate is off by one at most
-            int64_t k = (int64_t)((double)top / (double)sum);
-            const int64_t r = top - k * sum;
-            k += r < 0 ? -1 : r >= sum ? 1 : 0;
-            o = (uint32_t)k;
-          }
-          if (a.softmax && part == 0) a.softmax[at] = (int32_t)o;
-        }
-        s_raw[(3 * h) * VA_STRIDE + tid] = (unsigned char)o;
-        s_raw[(3 * h + 1) * VA_STRIDE + tid] = (unsigned char)(o >> 8);
-        s_raw[(3 * h + 2) * VA_STRIDE + tid] = (unsigned char)(o >> 16);
-        uint32_t warp_sum = __reduce_add_sync(~0u, o);  // at most 32 x 2^20
-        if (lane == 0 && warp_sum) atomicAdd(&s_total[h], (unsigned long long)warp_sum);
-      }
+    for (int j = 0; j < 8; j++) v[j] = queue[(stage * 8 + j) * 32];
+    uint2 d[NT];
 #pragma unroll
-      for (int k = 3 * HT; k < 8 * NT; k++) s_raw[k * VA_STRIDE + tid] = 0;
-    }
-    __syncthreads();
-    for (uint32_t k0 = wk * 32; k0 < VA_KEYS && base + k0 < last; k0 += groups * 32) {
-      uint4 v[8];
+    for (int k = 0; k < NT; k++) d[k] = *reinterpret_cast<const uint2*>(s_digits + (k * 8 + gl) * VA_STRIDE + k0 + 8 * t);
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int64_t at = s_at[k0 + 8 * t + j];
-        v[j] = in_row && at >= 0 ? load_once(c.v + at + byte) : make_uint4(0, 0, 0, 0);
-      }
-      uint2 d[NT];
+    for (int w = 0; w < 4; w++) {
+      uint32_t p[4], r[4];
+      auto word = [&](int j) { return w == 0 ? v[j].x : w == 1 ? v[j].y : w == 2 ? v[j].z : v[j].w; };
+      turn4(word(0), word(1), word(2), word(3), p);
+      turn4(word(4), word(5), word(6), word(7), r);
+      p[3] ^= 0x80808080u;
+      r[3] ^= 0x80808080u;
+      if (EB == 2) { p[1] ^= 0x80808080u; r[1] ^= 0x80808080u; }
 #pragma unroll
-      for (int k = 0; k < NT; k++) d[k] = *reinterpret_cast<const uint2*>(s_raw + (k * 8 + gl) * VA_STRIDE + k0 + 8 * t);
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        uint32_t p[4], r[4];
-        auto word = [&](int j) { return w == 0 ? v[j].x : w == 1 ? v[j].y : w == 2 ? v[j].z : v[j].w; };
-        turn4(word(0), word(1), word(2), word(3), p);
-        turn4(word(4), word(5), word(6), word(7), r);
-        p[3] ^= 0x80808080u;
-        r[3] ^= 0x80808080u;
-        if (EB == 2) { p[1] ^= 0x80808080u; r[1] ^= 0x80808080u; }
-#pragma unroll
-        for (int k = 0; k < NT; k++) {
-          mma_u8u8(acc[2 * w][k], p[0], p[1], r[0], r[1], d[k].x, d[k].y);
-          mma_u8u8(acc[2 * w + 1][k], p[2], p[3], r[2], r[3], d[k].x, d[k].y);
-        }
+      for (int k = 0; k < NT; k++) {
+        mma_u8u8(acc[2 * w][k], p[0], p[1], r[0], r[1], d[k].x, d[k].y);
+        mma_u8u8(acc[2 * w + 1][k], p[2], p[3], r[2], r[3], d[k].x, d[k].y);
       }
     }
+    fetch(k0 + 2 * groups * 32, stage);  // every register of this place has been used
+    stage ^= 1;
   }
+  copy_wait<0>();
 
   // weights of the byte planes in the lane; digits and the warps that dealt the keys through shared memory:
   // s_part[warp][column of eight][channel], eight columns at a time
-  int64_t* s_part = reinterpret_cast<int64_t*>(s_raw);
+  int64_t* s_part = reinterpret_cast<int64_t*>(s_dyn);
   const uint32_t outputs = a.v_split * ELEMS;  // channels of the block
-  constexpr int MINE = (HT * VA_THREADS / 32 * ELEMS + VA_THREADS - 1) / VA_THREADS;  // (head, channel) of a thread at most
+  constexpr int MINE = (HT * THREADS / 32 * ELEMS + THREADS - 1) / THREADS;  // (head, channel) of a thread at most
   uint64_t mine[MINE];
 #pragma unroll
   for (int i = 0; i < MINE; i++) mine[i] = 0;
@@ -504,7 +583,7 @@ __global__ void __launch_bounds__(VA_THREADS) k_kv_values(AttendArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MINE; i++) {
-      const uint32_t at = i * VA_THREADS + tid, h = at / outputs, ch = at % outputs;
+      const uint32_t at = i * THREADS + tid, h = at / outputs, ch = at % outputs;
       if (h < hn) {
         for (uint32_t r = 0; r < 3; r++) {
           const uint32_t col = 3 * h + r;
@@ -528,7 +607,7 @@ __global__ void __launch_bounds__(VA_THREADS) k_kv_values(AttendArgs a) {
   };
 #pragma unroll
   for (int i = 0; i < MINE; i++) {
-    const uint32_t at = i * VA_THREADS + tid, h = at / outputs, ch = ch0 + at % outputs;
+    const uint32_t at = i * THREADS + tid, h = at / outputs, ch = ch0 + at % outputs;
     if (h < hn && ch < D) {
       const uint64_t v = mine[i] - bias * (uint64_t)s_total[h], to = (row0 + h) * D + ch;
       if (used == 1) finish((int64_t)v, to);
@@ -543,7 +622,7 @@ __global__ void __launch_bounds__(VA_THREADS) k_kv_values(AttendArgs a) {
     __syncthreads();
     if (s_last) {
       __threadfence();
-      for (uint32_t at = tid; at < hn * outputs; at += VA_THREADS) {
+      for (uint32_t at = tid; at < hn * outputs; at += THREADS) {
         const uint32_t h = at / outputs, ch = ch0 + at % outputs;
         if (ch < D) finish(__ldcg(a.acc + (row0 + h) * D + ch), (row0 + h) * D + ch);
       }
@@ -553,18 +632,24 @@ __global__ void __launch_bounds__(VA_THREADS) k_kv_values(AttendArgs a) {
   if (chunk == 0 && part == 0 && tid < hn && a.sum[row0 + tid] == 0) kv_flag(c, STATUS_KV_EXP);
 }
 
-template <int EB>
-static int launch_scores(grape_ctx* ctx, const AttendArgs& a, uint32_t ht, uint32_t grid, uint32_t threads, size_t smem) {
-  auto kernel = ht == 1 ? k_kv_scores<EB, 1> : ht == 2 ? k_kv_scores<EB, 2> : ht == 4 ? k_kv_scores<EB, 4> : k_kv_scores<EB, 8>;
-  GRAPE_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SC_SMEM));
-  kernel<<<grid, threads, smem, ctx->stream>>>(a);
+template <class K>
+static int launch(grape_ctx* ctx, K kernel, const AttendArgs& a, uint64_t grid, uint32_t threads, size_t smem) {
+  if (smem > 48 * 1024) GRAPE_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kernel<<<(uint32_t)grid, threads, smem, ctx->stream>>>(a);
+  ctx->launches += 1;
   return GRAPE_OK;
 }
 
 template <int EB>
-static void launch_values(grape_ctx* ctx, const AttendArgs& a, uint32_t ht, uint32_t grid) {
-  auto kernel = ht == 1 ? k_kv_values<EB, 1> : ht == 2 ? k_kv_values<EB, 2> : ht == 5 ? k_kv_values<EB, 5> : k_kv_values<EB, 8>;
-  kernel<<<grid, VA_THREADS, 0, ctx->stream>>>(a);
+static int launch_scores(grape_ctx* ctx, const AttendArgs& a, uint32_t ht, uint64_t grid, uint32_t threads, size_t smem) {
+  return launch(ctx, ht == 1 ? k_kv_scores<EB, 1> : ht == 2 ? k_kv_scores<EB, 2> : ht == 4 ? k_kv_scores<EB, 4> : k_kv_scores<EB, 8>, a, grid, threads,
+                smem);
+}
+
+template <int EB>
+static int launch_values(grape_ctx* ctx, const AttendArgs& a, uint32_t ht, uint64_t grid) {
+  return launch(ctx, ht == 1 ? k_kv_values<EB, 1> : ht == 2 ? k_kv_values<EB, 2> : ht == 5 ? k_kv_values<EB, 5> : k_kv_values<EB, 8>, a, grid,
+                va_threads(ht), va_smem(ht));
 }
 
 static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs& a) {
@@ -579,12 +664,14 @@ static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs
   uint32_t ht = 1;
   while (ht < 8 && ht < a.group && (uint64_t)2 * ht * row_bytes * 8 <= SC_SMEM) ht *= 2;
   a.tiles = (a.group + ht - 1) / ht;
-  const uint32_t blks = (row_bytes + 63) / 64;
-  const size_t smem = (size_t)blks * ht * 512;
-  const uint32_t threads = smem > 64 * 1024 ? 512 : 256;
+  const uint32_t blks = (row_bytes + 63) / 64, mt = sc_sixteens(ht);
+  const size_t columns_bytes = (size_t)blks * ht * 512, queue_bytes = (size_t)sc_stages(ht) * mt * 1024, part_bytes = (size_t)2 * mt * ht * 64;
+  // columns that leave room for one block an SM: 16 warps instead of 8, where their queues still fit
+  const uint32_t threads = columns_bytes >= 48 * 1024 && columns_bytes + 16 * (queue_bytes + part_bytes) <= SC_SMEM_ALL ? 512 : 256;
   a.split = 1;
   while (a.split < threads / 32 && blks / (2 * a.split) >= 8) a.split *= 2;
-  const uint32_t step = threads / 32 / a.split * 16;
+  const size_t smem = columns_bytes + threads / 32 * (queue_bytes + (a.split > 1 ? part_bytes : 0));
+  const uint32_t step = threads / 32 / a.split * 16 * mt;
   uint64_t keys = std::max<uint64_t>(step, (256 * 1024 / row_bytes + step - 1) / step * step);
   while (keys > step && kv_rows * a.tiles * ((cols + keys - 1) / keys) < 4ull * sms) keys = std::max<uint64_t>(step, keys / 2 / step * step);
   a.chunk_keys = (uint32_t)keys;
@@ -594,16 +681,15 @@ static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs
   // the rest of the warps share the keys.
   const uint32_t v_ht = a.group == 1 ? 1 : a.group == 2 ? 2 : a.group <= 5 ? 5 : 8;
   a.v_tiles = (a.group + v_ht - 1) / v_ht;
-  const uint32_t segments = (row_bytes + 127) / 128;
+  const uint32_t segments = (row_bytes + 127) / 128, v_warps = va_threads(v_ht) / 32;
   a.v_split = 1;
-  while (a.v_split < VA_THREADS / 32 && a.v_split < segments) a.v_split *= 2;
+  while (a.v_split < v_warps && a.v_split < segments) a.v_split *= 2;
   a.v_parts = (segments + a.v_split - 1) / a.v_split;
-  const uint32_t v_step = VA_THREADS / 32 / a.v_split * 32;
-  uint64_t v_keys = std::max<uint64_t>(VA_KEYS, (256 * 1024 / (a.v_split * 128) + VA_KEYS - 1) / VA_KEYS * VA_KEYS);
-  while (v_keys > v_step && kv_rows * a.v_tiles * a.v_parts * ((cols + v_keys - 1) / v_keys) < 4ull * sms)
-    v_keys = std::max<uint64_t>(v_step, v_keys / 2 / v_step * v_step);
-  a.v_chunk_keys = (uint32_t)std::min<uint64_t>(v_keys, VA_MAX_CHUNK);
-  const uint64_t v_chunks = (cols + a.v_chunk_keys - 1) / a.v_chunk_keys;
+  const uint32_t v_step = v_warps / a.v_split * 32;
+  uint64_t v_keys = VA_CHUNK;
+  while (v_keys > v_step && kv_rows * a.v_tiles * a.v_parts * ((cols + v_keys - 1) / v_keys) < 4ull * sms) v_keys /= 2;
+  a.v_chunk_keys = (uint32_t)v_keys;
+  const uint64_t v_chunks = (cols + v_keys - 1) / v_keys;
 
   const uint64_t most = 0x7fffffffu;
   if (kv_rows * a.tiles * chunks > most || rows * exp_chunks > most || kv_rows * a.v_tiles * a.v_parts * v_chunks > most ||
@@ -613,12 +699,13 @@ static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs
   a.exp_chunks = (uint32_t)exp_chunks;
   a.v_chunks = (uint32_t)v_chunks;
   const uint64_t dones = kv_rows * a.v_tiles * a.v_parts;
-  a.done_per_tile = (uint32_t)((uint64_t)a.v_tiles * a.v_parts);  // zeroed by the first tile of a key head
+  a.done_per_row = (uint32_t)((uint64_t)a.v_tiles * a.v_parts);
+  a.valid_stride = (cols + 15) & ~uint64_t(15);
   auto up = [](uint64_t n) { return (n + 255) & ~uint64_t(255); };
-  const uint64_t b_max = up(rows * chunks * 4), b_acc = up(rows * D * 8), b_done = up(dones * 4), b_sum = a.sum ? 0 : up(rows * 8);
+  const uint64_t b_max = up(rows * chunks * 4), b_acc = up(rows * D * 8), b_done = up(dones * 4), b_valid = up(kv_rows * a.valid_stride), b_sum = a.sum ? 0 : up(rows * 8);
   const uint64_t b_keys = up(rows * a.max_keys * 4);
   void* w = nullptr;
-  if (int rc = kv_workspace(ctx, b_max + b_acc + b_done + b_sum + (a.score ? 0 : b_keys) + (a.exp_out ? 0 : b_keys), &w)) return rc;
+  if (int rc = kv_workspace(ctx, b_max + b_acc + b_done + b_valid + b_sum + (a.score ? 0 : b_keys) + (a.exp_out ? 0 : b_keys), &w)) return rc;
   char* p = reinterpret_cast<char*>(w);
   a.chunk_max = reinterpret_cast<int32_t*>(p);
   p += b_max;
@@ -626,17 +713,16 @@ static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs
   p += b_acc;
   a.done = reinterpret_cast<uint32_t*>(p);
   p += b_done;
+  a.valid = reinterpret_cast<unsigned char*>(p);
+  p += b_valid;
   if (!a.sum) { a.sum = reinterpret_cast<int64_t*>(p); p += b_sum; }
   if (!a.score) { a.score = reinterpret_cast<int32_t*>(p); p += b_keys; }
   if (!a.exp_out) { a.exp_out = reinterpret_cast<int32_t*>(p); p += b_keys; }
 
-  const uint32_t grid = (uint32_t)(kv_rows * a.tiles * chunks), v_grid = (uint32_t)(dones * v_chunks);
+  const uint64_t grid = kv_rows * a.tiles * chunks;
   if (int rc = cache->bits == 32 ? launch_scores<4>(ctx, a, ht, grid, threads, smem) : launch_scores<2>(ctx, a, ht, grid, threads, smem)) return rc;
-  if (cache->page_size % 4 == 0 && a.max_keys % 4 == 0) k_kv_exp<4><<<(uint32_t)(rows * exp_chunks), EX_THREADS, 0, ctx->stream>>>(a);
-  else k_kv_exp<1><<<(uint32_t)(rows * exp_chunks), EX_THREADS, 0, ctx->stream>>>(a);
-  if (cache->bits == 32) launch_values<4>(ctx, a, v_ht, v_grid);
-  else launch_values<2>(ctx, a, v_ht, v_grid);
-  ctx->launches += 3;
+  if (int rc = launch(ctx, k_kv_exp, a, rows * exp_chunks, EX_THREADS, 0)) return rc;
+  if (int rc = cache->bits == 32 ? launch_values<4>(ctx, a, v_ht, dones * v_chunks) : launch_values<2>(ctx, a, v_ht, dones * v_chunks)) return rc;
   GRAPE_CUDA_TRY(ctx, cudaGetLastError());
   return GRAPE_OK;
 }
