@@ -6,6 +6,8 @@
 #include <algorithm>
 #include <exception>
 
+#include <cooperative_groups.h>
+
 #include "kv.cuh"
 
 namespace grape {
@@ -23,27 +25,30 @@ struct AttendArgs {
   uint64_t max_keys;
   int32_t *out, *score, *score_rem, *exp_in, *exp_out, *softmax, *out_rem;
   int64_t* sum;
-  int32_t* chunk_max;  // [batch][heads][chunks]
-  int64_t* acc;        // [batch][heads][head_dim]
-  uint32_t* done;      // blocks of a key head's tile and part that have added to acc
-  uint32_t tiles, split, chunks, chunk_keys;  // scores: head tiles of a key head, warps of a row, blocks of a row
-  uint32_t exp_chunks;
-  uint32_t v_tiles, v_parts, v_split, v_chunks, v_chunk_keys;  // values: head tiles, parts of a row, warps of a part, ...
-  uint32_t done_per_row;
-  unsigned char* valid;   // [batch][kv_heads][columns]: 1 where a column holds a position
-  uint64_t valid_stride;
+  int32_t* piece_max;      // [row + block of the grid][heads of a tile]: the largest score of a row's piece
+  uint32_t* before;        // [batch + 1]: key sets of the sequences before
+  int64_t* acc;            // [batch][heads][head_dim]
+  uint32_t* done;          // warps that have added to acc, per (row, part of a row's values, unit of a block)
+  unsigned char* valid;    // [batch][kv_heads][padded columns]: 1 where a column holds a position
+  int64_t* row_at;         // [batch][kv_heads][padded columns]: offset of a column's key and value (of some row where there is none)
+  unsigned char* digits;   // [batch][heads][3][padded columns]: the softmax in bytes
+  int64_t* weight;         // [batch][heads]: sum of the softmax
+  uint64_t padded, acc_count, done_count;
+  uint32_t tiles, split, stages;                       // scores: head tiles of a key head, warps of a row, stages of a queue
+  uint32_t score_grid, score_heads, score_keys;
+  uint32_t v_tiles, v_parts, v_split, v_heads;         // values: head tiles, parts of a row, segments of a part, heads of a tile
 };
 
 // Columns of a row that can hold a position: its length, or the slots of the selected pages.
-__device__ __forceinline__ uint32_t columns(const AttendArgs& a, uint32_t b, bool report) {
-  const uint32_t n = kv_length(a.c, a.len, b, a.selected ? ~0ull : a.max_keys, report);
+__device__ __forceinline__ uint32_t columns(const AttendArgs& a, uint32_t n) {
   if (!a.selected) return n;
-  if (n == 0) return 0;
-  const uint64_t all = (uint64_t)a.n_select * a.c.page_size;
-  return (uint32_t)min(all, a.max_keys);
+  return n == 0 ? 0 : (uint32_t)min((uint64_t)a.n_select * a.c.page_size, a.max_keys);
+}
+__device__ __forceinline__ uint32_t length(const AttendArgs& a, uint32_t b, bool report) {
+  return kv_length(a.c, a.len, b, a.selected ? ~0ull : a.max_keys, report);
 }
 
-// Page and slot of column i, or page -1 where the column holds no position.
+// Page and slot of column i of a sequence of n tokens, or page -1 where the column holds no position.
 __device__ __forceinline__ int32_t column_page(const AttendArgs& a, uint32_t b, uint32_t g, uint32_t n, uint32_t i, uint32_t& slot,
                                                bool report) {
   const KvView& c = a.c;
@@ -64,11 +69,70 @@ __device__ __forceinline__ int32_t column_page(const AttendArgs& a, uint32_t b, 
   return page;
 }
 
-// A lane's own queue in shared memory: 16-byte copies from global memory that this lane alone reads back, so
-// that no barrier is needed, only the wait for its own copies, and what is under way costs no registers.
-__device__ __forceinline__ void copy_async(uint4* to, const char* from, bool there) {
-  // nothing is read where `there` is false: the 16 bytes become zero
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
+// ---- how scores and values are split --------------------------------------------------------------
+// The rows (sequence, key head, head tile, ...) are laid end to end, each cut into sets of 16 or 32 keys, and
+// every block of the grid takes one span of sets, the same number for all: however ragged the lengths, the
+// blocks end together.  A block walks the pieces of the rows that its span covers.  Pieces of row r in block i
+// are numbered r + i: unique, and the pieces of a row lie together.
+constexpr uint32_t AT_BATCH = 256;  // sequences of a launch
+constexpr uint32_t AT_SMEM = 110 * 1024;     // dynamic shared memory of a block that shares its SM with another
+constexpr uint32_t AT_SMEM_ALONE = 222 * 1024;
+
+// s_before[b] = sets of the rows of the sequences before b; returns all of them.
+__device__ __forceinline__ uint32_t plan_sets(const AttendArgs& a, uint32_t* s_before, uint32_t keys, uint32_t rows, bool report) {
+  for (uint32_t b = threadIdx.x; b < a.c.batch; b += blockDim.x)
+    s_before[b + 1] = (columns(a, length(a, b, report)) + keys - 1) / keys * rows;
+  if (threadIdx.x == 0) s_before[0] = 0;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    uint32_t carry = 0;
+    for (uint32_t base = 0; base < a.c.batch; base += 32) {
+      const uint32_t b = base + threadIdx.x;
+      uint32_t v = b < a.c.batch ? s_before[b + 1] : 0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(~0u, v, o);
+        if ((int)threadIdx.x >= o) v += u;
+      }
+      if (b < a.c.batch) s_before[b + 1] = carry + v;
+      carry += __shfl_sync(~0u, v, 31);
+    }
+  }
+  __syncthreads();
+  return s_before[a.c.batch];
+}
+
+struct Piece {
+  uint32_t b, row, sets;         // sequence, row within it, key sets of the whole row
+  uint32_t first_set, count;     // the piece
+  uint32_t begin;                // of the row among all sets
+};
+__device__ __forceinline__ Piece piece_at(const AttendArgs& a, const uint32_t* s_before, uint32_t rows, uint32_t at, uint32_t end) {
+  uint32_t lo = 0, hi = a.c.batch;  // the last b with s_before[b] <= at
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (s_before[mid] <= at) lo = mid; else hi = mid;
+  }
+  Piece p;
+  p.b = lo;
+  p.sets = (s_before[lo + 1] - s_before[lo]) / rows;
+  p.row = (at - s_before[lo]) / p.sets;
+  p.begin = s_before[lo] + p.row * p.sets;
+  p.first_set = at - p.begin;
+  p.count = min(p.sets - p.first_set, end - at);
+  return p;
+}
+
+// ---- copies ------------------------------------------------------------------------------------------
+// A lane's own queue in shared memory: asynchronous copies that this lane alone reads back, so that no barrier
+// is needed, only the wait for its own copies, and what is under way costs no registers.  What the warps of an
+// SM have under way (about 150 KB) is what carries the kernels: one step at a time in registers (64 KB) gave
+// 3 TB/s.  Whole rows by bulk copies of one warp for all gave 3.4 TB/s, the same copies by a warp's lanes 3.1 to
+// 4.3: the issuing warps could not keep up.
+__device__ __forceinline__ void copy_async(void* to, const char* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async_8(void* to, const unsigned char* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -94,106 +158,109 @@ __device__ __forceinline__ void mma_u8u8(int32_t (&c)[4], uint32_t a0, uint32_t 
 //   q . k = sum_c 256^c (k' bytes . column c) - bias sum_d q_d,      c = 0 .. 7
 // and the eight weights are the eight columns of an m16n8k32: 16 keys, 32 bytes of each, one head.  A sum
 // of a column is at most 4096 elements x 4 bytes x 255 x 128 < 2^31.
-// A warp takes 16 keys (rows g and g + 8 of a lane), 64 bytes of them per step: a lane's 16 bytes are the A
-// registers of two instructions, no shuffles, no staging.  The columns (8 words per 4 bytes of a key) are
-// built once per block in shared memory.
 // What bounds it: bytes of the keys.  The instruction takes 2 cycles of an SM (measured, 570 T products/s) for
 // 512 bytes of keys and a head, which arrive every 22 cycles.
-constexpr int SC_MAX_THREADS = 512;
-constexpr int SC_SMEM = 128 * 1024;      // bytes of a block's columns at most
-constexpr int SC_SMEM_ALL = 224 * 1024;  // and of all that it keeps in shared memory
-
+// Columns 0..7 of the bytes of a word: byte p of column c is digit c - p of the element (two elements a word when
+// they have 16 bits).  u = q + 0x80808080: its four low bytes are the digits + 128, its fifth the fifth digit.
 template <int EB>
-__device__ __forceinline__ uint32_t column_word(const uint64_t (&u)[4 / EB], int c) {
-  // u: q + 0x80808080 per element, whose bytes are the digits + 128 and whose fifth byte is the fifth digit
-  uint32_t w = 0;
+__device__ __forceinline__ void column_words(const uint64_t (&u)[4 / EB], uint32_t (&w)[8]) {
+  uint32_t d[4 / EB], top[4 / EB];
 #pragma unroll
   for (int e = 0; e < 4 / EB; e++) {
-#pragma unroll
-    for (int p = 0; p < EB; p++) {
-      const int r = c - p;
-      if (r >= 0 && r <= 4) {
-        uint32_t digit = (uint32_t)(u[e] >> (8 * r)) & 0xffu;
-        if (r < 4) digit ^= 0x80u;
-        w |= digit << (8 * (e * EB + p));
-      }
-    }
+    d[e] = (uint32_t)u[e] ^ 0x80808080u;
+    top[e] = (uint32_t)(u[e] >> 32);  // bytes 5..7 of the pair (d, top) are zero
   }
-  return w;
+  if (EB == 4) {
+    w[0] = __byte_perm(d[0], top[0], 0x5550);
+    w[1] = __byte_perm(d[0], top[0], 0x5501);
+    w[2] = __byte_perm(d[0], top[0], 0x5012);
+    w[3] = __byte_perm(d[0], top[0], 0x0123);
+    w[4] = __byte_perm(d[0], top[0], 0x1234);
+    w[5] = __byte_perm(d[0], top[0], 0x2345);
+    w[6] = __byte_perm(d[0], top[0], 0x3455);
+    w[7] = __byte_perm(d[0], top[0], 0x4555);
+  } else {
+    constexpr uint32_t pick[8] = {0x5550, 0x5501, 0x5512, 0x5523, 0x5534, 0x5545, 0x5555, 0x5555};
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+      w[c] = __byte_perm(__byte_perm(d[0], top[0], pick[c]), __byte_perm(d[4 / EB - 1], top[4 / EB - 1], pick[c]), 0x5410);
+  }
 }
 
-__host__ __device__ constexpr int sc_sixteens(int ht) { return ht >= 4 ? 2 : 1; }  // sixteens of keys that share a read of the columns
-__host__ __device__ constexpr int sc_stages(int ht) { return ht >= 4 ? 4 : 5; }    // steps in a lane's queue
 
-template <int EB, int HT>
-__global__ void __launch_bounds__(SC_MAX_THREADS) k_kv_scores(AttendArgs a) {
-  constexpr int MT = sc_sixteens(HT), STAGES = sc_stages(HT);
-  constexpr int NV = 2 * MT * HT;               // values of a lane group: (head, eight of keys)
-  constexpr int OWN = NV >= 4 ? NV / 4 : 1;     // those that a lane finishes
-  constexpr int HEADS = HT >= 4 ? HT / 4 : 1;   // and the heads they belong to
-  extern __shared__ uint4 s_w[];  // [blk][HT][32 lanes]: 4 words, the columns of a lane's 16 bytes; the lanes' queues; partial sums
+constexpr uint32_t SC_SLAB = 1024;  // bytes of a warp's slab of sums
+// A step: 64 bytes of 32 keys (MT = 2), or of 16 where a row is shared by the warps of a block.
+__host__ __device__ constexpr int sc_stages(int mt) { return mt == 2 ? 5 : 4; }
+__host__ __device__ constexpr uint32_t sc_warp(int mt) { return sc_stages(mt) * mt * 1024 + SC_SLAB; }
+
+// MT: sixteens of keys of a set.  HT: heads of a tile.  A block builds the columns of a piece's tile; its warps (a
+// team of `split` where rows are long, each a part of the row) take the sets in turn.
+template <int EB, int HT, int MT>
+__global__ void __launch_bounds__(MT == 2 ? 256 : 512) k_kv_scores(AttendArgs a) {
+  constexpr int SLABS = HT * MT >= 2 ? HT * MT / 2 : 1;  // (head, key) pairs in 32s
+  constexpr uint32_t KEYS = 16 * MT;
+  constexpr int STAGES = sc_stages(MT);
+  extern __shared__ uint4 s_dyn[];  // columns, [blk][HT][32 lanes]: 4 words, those of a lane's 16 bytes; the warps' queues and slabs
   __shared__ unsigned long long s_bias[HT];
   __shared__ int32_t s_max[HT];
-  __shared__ unsigned char s_valid[SC_MAX_THREADS / 32][16 * MT];
+  __shared__ uint32_t s_before[AT_BATCH + 1];
   const KvView& c = a.c;
   const uint32_t D = c.head_dim, row_bytes = D * EB, blks = (row_bytes + 63) / 64;
-  uint32_t x = blockIdx.x;
-  const uint32_t tile = x % a.tiles;
-  x /= a.tiles;
-  const uint32_t chunk = x % a.chunks, row = x / a.chunks, g = row % c.kv_heads, b = row / c.kv_heads;
-  const uint32_t h0 = g * a.group + tile * HT, hn = min((uint32_t)HT, a.group - tile * HT);
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-  const uint32_t n = kv_length(c, a.len, b, a.selected ? ~0ull : a.max_keys, false);
-  const uint32_t cols = columns(a, b, chunk == 0 && tid == 0);
-  const uint64_t row0 = (uint64_t)b * a.heads + h0;  // first of the block's rows
-  if (chunk == 0) {
-    // what the later passes add to
-    for (uint32_t i = tid; i < hn * D; i += blockDim.x) a.acc[row0 * D + i] = 0;
-    for (uint32_t i = tid; i < hn; i += blockDim.x) a.sum[row0 + i] = 0;
-    for (uint32_t i = tid; tile == 0 && i < a.done_per_row; i += blockDim.x) a.done[(uint64_t)row * a.done_per_row + i] = 0;
-    if (cols == 0) {
-      for (uint32_t i = tid; i < hn * D; i += blockDim.x) {
-        a.out[row0 * D + i] = 0;
-        if (a.out_rem) a.out_rem[row0 * D + i] = 0;
-      }
-    }
-  }
-  const uint32_t first = chunk * a.chunk_keys, last = min(cols, first + a.chunk_keys);
-  if (first >= last) return;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t = lane & 3;
+  const uint32_t rows = c.kv_heads * a.tiles, split = MT == 2 ? 1 : a.split, teams = (blockDim.x >> 5) / split;
+  const uint32_t wd = warp % split, team = warp / split, blk0 = blks * wd / split, blk1 = blks * (wd + 1) / split;
+  const uint32_t total = plan_sets(a, s_before, KEYS, rows, blockIdx.x == 0);
+  const uint32_t span = (total + gridDim.x - 1) / gridDim.x;
+  const uint32_t begin = min(total, blockIdx.x * span), end = min(total, begin + span);
 
-  const uint32_t gl = lane >> 2, t = lane & 3;
-  const uint32_t wd = warp % a.split, wk = warp / a.split, keys_at_once = warps / a.split * 16 * MT;
-  const uint32_t blk0 = blks * wd / a.split, blk1 = blks * (wd + 1) / a.split;
-
-  // A step is 64 bytes of the warp's 16 MT keys.  `fetch` walks the steps STAGES - 1 ahead of their use; which of
-  // a lane's keys exist goes through `fifo`, four bits for each set of keys under way.
-  uint4* const queue = s_w + (uint64_t)blks * HT * 32 + (uint64_t)warp * STAGES * MT * 64 + lane;
+  // `fetch` walks the warp's steps STAGES - 1 ahead of their use, through the sets of a piece and on to the next.  A
+  // column that holds no position reads some other row of the cache and is dropped at the end; `fifo` has a bit
+  // for this lane's key of every set under way.
+  char* const mine = reinterpret_cast<char*>(s_dyn + (uint64_t)blks * HT * 32) + (uint64_t)warp * sc_warp(MT);
+  uint4* const queue = reinterpret_cast<uint4*>(mine) + lane;
+  Piece ahead = {};
+  uint32_t ahead_at = begin, ahead_k = team, ahead_blk = blk0, ahead_stage = 0, fifo = 0, under_way = 0;
   const char* key[2 * MT];
-  uint32_t ahead_base = first, ahead_blk = blk0, ahead_slot = 0, fifo = 0, under_way = 0;
+  auto settle = [&]() {  // on to the piece that holds the warp's next set
+    while (ahead_at < end && ahead_k >= ahead.count) {
+      ahead_at += ahead.count;
+      ahead_k = team;
+      if (ahead_at < end) ahead = piece_at(a, s_before, rows, ahead_at, end);
+    }
+  };
+  if (begin < end) ahead = piece_at(a, s_before, rows, begin, end);
+  settle();
   auto fetch = [&]() {
-    if (ahead_base < last) {
+    if (ahead_at < end) {
       if (ahead_blk == blk0) {
-        uint32_t mask = 0;
+        const uint32_t g = ahead.row / a.tiles, tile = ahead.row % a.tiles, n = length(a, ahead.b, false), cols = columns(a, n);
+        const uint32_t i = (ahead.first_set + ahead_k) * KEYS + (lane & (KEYS - 1));
+        uint32_t slot = 0;
+        int32_t page = i < cols ? column_page(a, ahead.b, g, n, i, slot, tile == 0 && wd == 0) : -1;
+        fifo |= (page >= 0 ? 1u : 0u) << under_way++;
+        const bool first = tile == 0 && wd == 0 && lane < KEYS;
+        const uint64_t note = ((uint64_t)ahead.b * c.kv_heads + g) * a.padded + i;
+        if (first) a.valid[note] = page >= 0;
+        if (page < 0) page = slot = 0;
+        const int64_t offset = page * c.page_stride + g * c.head_stride + slot * c.slot_stride;
+        if (first) a.row_at[note] = offset;
+        // the values' pass takes 32 keys at a time: what lies behind an odd last sixteen is some row too
+        const uint32_t set = ahead.first_set + ahead_k;
+        if (KEYS == 16 && tile == 0 && wd == 0 && lane >= 16 && set % 2 == 0 && (set + 1) * 16 >= cols)
+          a.row_at[((uint64_t)ahead.b * c.kv_heads + g) * a.padded + set * 16 + lane] = g * c.head_stride;
+        const uint64_t row = reinterpret_cast<uint64_t>(c.k + offset);
 #pragma unroll
-        for (int m = 0; m < 2 * MT; m++) {
-          const uint32_t i = ahead_base + wk * 16 * MT + m * 8 + gl;
-          uint32_t slot;
-          const int32_t page = i < last ? column_page(a, b, g, n, i, slot, t == 0 && wd == 0) : -1;
-          key[m] = page >= 0 ? c.k + page * c.page_stride + g * c.head_stride + slot * c.slot_stride + t * 16 : nullptr;
-          if (page >= 0) mask |= 1u << m;
-        }
-        fifo |= mask << (4 * under_way++);
+        for (int m = 0; m < 2 * MT; m++) key[m] = reinterpret_cast<const char*>(__shfl_sync(~0u, row, m * 8 + gl)) + t * 16;
       }
-      const bool in = ahead_blk * 64 + t * 16 < row_bytes;
+      if (ahead_blk * 64 + t * 16 < row_bytes) {
 #pragma unroll
-      for (int m = 0; m < 2 * MT; m++) {
-        const bool there = in && key[m];
-        copy_async(queue + (ahead_slot * 2 * MT + m) * 32, there ? key[m] + ahead_blk * 64 : c.k, there);
+        for (int m = 0; m < 2 * MT; m++) copy_async(queue + (ahead_stage * 2 * MT + m) * 32, key[m] + ahead_blk * 64);
       }
-      ahead_slot = ahead_slot + 1 == STAGES ? 0 : ahead_slot + 1;
+      ahead_stage = ahead_stage + 1 == STAGES ? 0 : ahead_stage + 1;
       if (++ahead_blk == blk1) {
         ahead_blk = blk0;
-        ahead_base += keys_at_once;
+        ahead_k += teams;
+        settle();
       }
     }
     copy_commit();
@@ -201,226 +268,319 @@ __global__ void __launch_bounds__(SC_MAX_THREADS) k_kv_scores(AttendArgs a) {
 #pragma unroll 1
   for (int i = 0; i < STAGES - 1; i++) fetch();
 
-  // the operand columns, and the sum of each head's query
-  if (tid < HT) { s_bias[tid] = 0; s_max[tid] = INT32_MIN; }
-  __syncthreads();
   {
-    constexpr uint32_t PER = 4 / EB;  // elements of a word
-    const uint32_t share = blockDim.x / HT, h = tid / share;
-    const int32_t* q = a.q + (uint64_t)b * a.q_stride + (uint64_t)(h0 + h) * D;
-    int64_t total = 0;
-    for (uint32_t i = tid % share; i < blks * 16; i += share) {
-      uint64_t u[PER];
-#pragma unroll
-      for (uint32_t e = 0; e < PER; e++) {
-        const uint32_t d = i * PER + e;
-        const int32_t v = h < hn && d < D ? __ldg(q + d) : 0;
-        total += v;
-        u[e] = (uint64_t)((int64_t)v + 0x80808080ll);
+    // what the later passes add to, the plan, and the rows that have no column
+    const uint64_t at = (uint64_t)blockIdx.x * blockDim.x + tid, step = (uint64_t)gridDim.x * blockDim.x;
+    for (uint64_t i = at; i < a.acc_count; i += step) a.acc[i] = 0;
+    for (uint64_t i = at; i < a.done_count; i += step) a.done[i] = 0;
+    for (uint64_t i = at; i < (uint64_t)c.batch * a.heads; i += step) a.weight[i] = 0;
+    for (uint64_t i = at; i <= c.batch; i += step) a.before[i] = s_before[i];
+    for (uint32_t b = 0; b < c.batch; b++) {
+      if (s_before[b] != s_before[b + 1]) continue;
+      for (uint64_t i = at; i < (uint64_t)a.heads * D; i += step) {
+        a.out[(uint64_t)b * a.heads * D + i] = 0;
+        if (a.out_rem) a.out_rem[(uint64_t)b * a.heads * D + i] = 0;
+        if (i < a.heads) a.sum[(uint64_t)b * a.heads + i] = 0;
       }
-      // word i of the row: block i / 16, lane group (i / 4) % 4, word i % 4
-      uint32_t* to = reinterpret_cast<uint32_t*>(s_w + ((uint64_t)(i / 16) * HT + h) * 32 + (i / 4) % 4) + i % 4;
-#pragma unroll
-      for (int k = 0; k < 8; k++) to[k * 16] = column_word<EB>(u, k);
     }
-    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
-    if (lane == 0) atomicAdd(&s_bias[h], (unsigned long long)total);
   }
-  __syncthreads();
 
-  const uint64_t bias = EB == 4 ? uint64_t(1) << 31 : uint64_t(1) << 15;
-  constexpr uint32_t FLIP = EB == 4 ? 0x80000000u : 0x80008000u;
-  int32_t best[HEADS];
-#pragma unroll
-  for (int j = 0; j < HEADS; j++) best[j] = INT32_MIN;
+  uint32_t stage = 0;
   bool range = false;
-  auto finish = [&](uint64_t acc, uint32_t h, uint32_t i) {
-    acc -= bias * (uint64_t)s_bias[h];
-    const int64_t s = rdiv((int64_t)acc, a.score_shift);
-    const int32_t v = saturate(s, INT32_MIN, INT32_MAX, range);
-    const uint64_t at = (row0 + h) * a.max_keys + i;
-    a.score[at] = v;
-    if (a.score_rem) a.score_rem[at] = (int32_t)(uint32_t)(acc - ((uint64_t)s << a.score_shift));
-    return v;
-  };
-
-  uint32_t slot = 0;
-  for (uint32_t base = first; base < last; base += keys_at_once) {
-    int32_t acc[HT][MT][4];
+  for (uint32_t at = begin; at < end;) {
+    const Piece p = piece_at(a, s_before, rows, at, end);
+    const uint32_t g = p.row / a.tiles, tile = p.row % a.tiles;
+    const uint32_t h0 = g * a.group + tile * HT, hn = min((uint32_t)HT, a.group - tile * HT);
+    const uint64_t row0 = (uint64_t)p.b * a.heads + h0;
+    // the operand columns, and the sum of each head's query
+    if (tid < HT) { s_bias[tid] = 0; s_max[tid] = INT32_MIN; }
+    __syncthreads();
+    {
+      constexpr uint32_t PER = 4 / EB;  // elements of a word
+      const uint32_t share = blockDim.x / HT, h = tid / share;
+      const int32_t* q = a.q + (uint64_t)p.b * a.q_stride + (uint64_t)(h0 + h) * D;
+      int64_t sum = 0;
+      for (uint32_t i = tid % share; i < blks * 16; i += share) {
+        uint64_t u[PER];
 #pragma unroll
-    for (int h = 0; h < HT; h++)
+        for (uint32_t e = 0; e < PER; e++) {
+          const uint32_t d = i * PER + e;
+          const int32_t v = h < hn && d < D ? __ldg(q + d) : 0;
+          sum += v;
+          u[e] = (uint64_t)((int64_t)v + 0x80808080ll);
+        }
+        // word i of the row: block i / 16, lane group (i / 4) % 4, word i % 4
+        uint32_t* to = reinterpret_cast<uint32_t*>(s_dyn + ((uint64_t)(i / 16) * HT + h) * 32 + (i / 4) % 4) + i % 4;
+        uint32_t w[8];
+        column_words<EB>(u, w);
 #pragma unroll
-      for (int m = 0; m < MT; m++) acc[h][m][0] = acc[h][m][1] = acc[h][m][2] = acc[h][m][3] = 0;
-#pragma unroll 1
-    for (uint32_t blk = blk0; blk < blk1; blk++) {
-      copy_wait<STAGES - 2>();
-      uint4 y[2 * MT];
-#pragma unroll
-      for (int m = 0; m < 2 * MT; m++) {
-        y[m] = queue[(slot * 2 * MT + m) * 32];
-        y[m].x ^= FLIP;
-        y[m].y ^= FLIP;
-        y[m].z ^= FLIP;
-        y[m].w ^= FLIP;
+        for (int k = 0; k < 8; k++) to[k * 16] = w[k];
       }
-      slot = slot + 1 == STAGES ? 0 : slot + 1;
-      fetch();  // into the place that was read a step ago
-      const uint4* w = s_w + (uint64_t)blk * HT * 32 + lane;
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+      if (lane == 0) atomicAdd(&s_bias[h], (unsigned long long)sum << (EB == 4 ? 31 : 15));
+    }
+    __syncthreads();
+
+    int32_t best[SLABS];
 #pragma unroll
-      for (int h = 0; h < HT; h++) {
-        if (HT > 2 && h >= hn) break;
-        const uint4 z = w[h * 32];
+    for (int j = 0; j < SLABS; j++) best[j] = INT32_MIN;
+    // teams of several warps meet in every set: all of a block's teams take the same number of turns
+    for (uint32_t k = team; k < (split == 1 ? p.count : (p.count + teams - 1) / teams * teams); k += teams) {
+      const bool real = split == 1 || k < p.count;
+      int32_t acc[HT][MT][4];
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-          mma_u8s8(acc[h][m], y[2 * m].x, y[2 * m + 1].x, y[2 * m].y, y[2 * m + 1].y, z.x, z.y);
-          mma_u8s8(acc[h][m], y[2 * m].z, y[2 * m + 1].z, y[2 * m].w, y[2 * m + 1].w, z.z, z.w);
+      for (int h = 0; h < HT; h++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) acc[h][m][0] = acc[h][m][1] = acc[h][m][2] = acc[h][m][3] = 0;
+      if (real) {
+#pragma unroll 1
+        for (uint32_t blk = blk0; blk < blk1; blk++) {
+          constexpr uint32_t FLIP = EB == 4 ? 0x80000000u : 0x80008000u;
+          copy_wait<STAGES - 2>();
+          uint4 y[2 * MT];
+#pragma unroll
+          for (int m = 0; m < 2 * MT; m++) {
+            y[m] = queue[(stage * 2 * MT + m) * 32];
+            y[m].x ^= FLIP;
+            y[m].y ^= FLIP;
+            y[m].z ^= FLIP;
+            y[m].w ^= FLIP;
+          }
+          stage = stage + 1 == STAGES ? 0 : stage + 1;
+          fetch();  // into the place that was read a step ago
+          const uint4* w = s_dyn + (uint64_t)blk * HT * 32 + lane;
+#pragma unroll
+          for (int h = 0; h < HT; h++) {
+            if (HT > 2 && h >= hn) break;
+            const uint4 z = w[h * 32];
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+              mma_u8s8(acc[h][m], y[2 * m].x, y[2 * m + 1].x, y[2 * m].y, y[2 * m + 1].y, z.x, z.y);
+              mma_u8s8(acc[h][m], y[2 * m].z, y[2 * m + 1].z, y[2 * m].w, y[2 * m + 1].w, z.z, z.w);
+            }
+          }
         }
       }
-    }
-    const uint32_t mask = fifo & 15;
-    fifo >>= 4;
-    under_way--;
-    // Lane (g, t) holds columns 2t and 2t + 1 of keys g and g + 8.  The sum over t leaves lane t with the values
-    // t OWN .. of (head * MT + sixteen) * 2 + eight: each lane finishes its own.
-    uint64_t v[NV];
-#pragma unroll
-    for (int h = 0; h < HT; h++)
-#pragma unroll
-      for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-          v[(h * MT + m) * 2 + e] = ((uint64_t)(int64_t)acc[h][m][2 * e] + ((uint64_t)(int64_t)acc[h][m][2 * e + 1] << 8)) << (16 * t);
-    if (NV >= 4) {
-#pragma unroll
-      for (int j = 0; j < NV / 2; j++) {
-        const uint64_t keep = t & 2 ? v[j + NV / 2] : v[j], give = t & 2 ? v[j] : v[j + NV / 2];
-        v[j] = keep + __shfl_xor_sync(~0u, give, 2);
+      bool there = false;
+      if (real) {
+        there = fifo & 1;
+        fifo >>= 1;
+        under_way--;
       }
-    } else {
-      v[0] += __shfl_xor_sync(~0u, v[0], 2);
-      v[1] += __shfl_xor_sync(~0u, v[1], 2);
-    }
+      const uint32_t i = (p.first_set + k) * KEYS + (lane & (KEYS - 1));
+      // Lane (g, t) holds columns 2t and 2t + 1 of keys g and g + 8.  Through a slab of shared memory the eight sums
+      // of a (head, key) come to one lane, the lane of the key; warps that share a row add theirs up on the way
+      // (a column's sum over the whole row stays below 2^31).
 #pragma unroll
-    for (int j = 0; j < OWN; j++) {
-      const uint64_t keep = t & 1 ? v[j + OWN] : v[j], give = t & 1 ? v[j] : v[j + OWN];
-      v[j] = keep + __shfl_xor_sync(~0u, give, 1);
-    }
-    const uint32_t own0 = NV >= 4 ? t * OWN : t & 1, key0 = base + wk * 16 * MT + gl;
-    if (tile == 0 && wd == 0 && t < 2 * MT && key0 + t * 8 < last) a.valid[(uint64_t)row * a.valid_stride + key0 + t * 8] = (mask >> t) & 1;
-    if (a.split == 1) {
+      for (int j = 0; j < SLABS; j++) {
+        int2* slab = reinterpret_cast<int2*>(mine + sc_warp(MT) - SC_SLAB);
 #pragma unroll
-      for (int j = 0; j < OWN; j++) {
-        const uint32_t own = own0 + j, h = own / (2 * MT), e = own % (2 * MT);
-        if (h < hn && (NV >= 4 || t < 2) && ((mask >> e) & 1)) best[j * HEADS / OWN] = max(best[j * HEADS / OWN], finish(v[j], h, key0 + e * 8));
-      }
-    } else {
-      // warps that share the keys add up in shared memory, [warp][value][g]
-      int64_t* s_part = reinterpret_cast<int64_t*>(s_w + (uint64_t)blks * HT * 32 + (uint64_t)warps * STAGES * MT * 64);
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < OWN; j++)
-        if (NV >= 4 || t < 2) s_part[((uint64_t)warp * NV + own0 + j) * 8 + gl] = (int64_t)v[j];
-      if (wd == 0 && t < 2 * MT) s_valid[wk][t * 8 + gl] = (mask >> t) & 1;
-      __syncthreads();
-      for (uint32_t i = wd * 32 + lane; i < NV * 8; i += a.split * 32) {
-        const uint32_t own = i / 8, h = own / (2 * MT), at = own % (2 * MT) * 8 + i % 8;
-        if (h >= hn || !s_valid[wk][at]) continue;
-        uint64_t sum = 0;
-        for (uint32_t w = 0; w < a.split; w++) sum += (uint64_t)s_part[((uint64_t)(wk * a.split + w) * NV + own) * 8 + i % 8];
-        atomicMax(&s_max[h], finish(sum, h, base + wk * 16 * MT + at));
+        for (int z = 0; z < (HT * MT >= 2 ? 4 : 2); z++) {
+          const int h = MT == 2 ? j : 2 * j + z / 2, m = MT == 2 ? z / 2 : 0, e = z % 2;
+          slab[(z * 8 + gl) * 4 + t] = make_int2(acc[h][m][2 * e], acc[h][m][2 * e + 1]);
+        }
+        if (split == 1) __syncwarp(); else __syncthreads();
+        if (split == 1 || j % split == wd) {
+          int32_t v[8] = {};
+          for (uint32_t w = 0; w < split; w++) {
+            const int4* from = reinterpret_cast<const int4*>(mine + ((int32_t)(team * split + w) - (int32_t)warp) * (int32_t)sc_warp(MT) + sc_warp(MT) - SC_SLAB) + lane * 2;
+            const int4 p0 = from[0], p1 = from[1];
+            v[0] += p0.x; v[1] += p0.y; v[2] += p0.z; v[3] += p0.w;
+            v[4] += p1.x; v[5] += p1.y; v[6] += p1.z; v[7] += p1.w;
+          }
+          const uint32_t h = MT == 2 ? j : 2 * j + lane / 16;
+          if (h < hn && there && (HT * MT >= 2 || lane < 16)) {
+            const int64_t v01 = (int64_t)v[0] + (int64_t)v[1] * 256, v23 = (int64_t)v[2] + (int64_t)v[3] * 256;
+            const int64_t v45 = (int64_t)v[4] + (int64_t)v[5] * 256, v67 = (int64_t)v[6] + (int64_t)v[7] * 256;
+            const uint64_t sum = (uint64_t)v01 + ((uint64_t)v23 << 16) + ((uint64_t)v45 << 32) + ((uint64_t)v67 << 48) - s_bias[h];
+            const int64_t quotient = rdiv((int64_t)sum, a.score_shift);
+            const int32_t score = saturate(quotient, INT32_MIN, INT32_MAX, range);
+            const uint64_t to = (row0 + h) * a.max_keys + i;
+            a.score[to] = score;
+            if (a.score_rem) a.score_rem[to] = (int32_t)(uint32_t)(sum - ((uint64_t)quotient << a.score_shift));
+            best[j] = max(best[j], score);
+          }
+        }
+        if (split == 1) __syncwarp(); else __syncthreads();
       }
     }
+    // the piece's largest score per head
+#pragma unroll
+    for (int j = 0; j < SLABS; j++) {
+      for (int o = MT == 2 ? 16 : 8; o; o >>= 1) best[j] = max(best[j], __shfl_xor_sync(~0u, best[j], o));
+      const uint32_t h = MT == 2 ? j : 2 * j + lane / 16;
+      if (lane % KEYS == 0 && h < HT) atomicMax(&s_max[h], best[j]);
+    }
+    __syncthreads();
+    if (tid < HT) a.piece_max[((uint64_t)p.b * rows + p.row + blockIdx.x) * HT + tid] = s_max[tid];
+    at += p.count;
   }
+  copy_wait<0>();
   if (range) kv_flag(c, STATUS_KV_RANGE);
-  if (a.split == 1) {
-#pragma unroll
-    for (int j = 0; j < HEADS; j++) {
-      for (int o = 16; o >= 4; o >>= 1) best[j] = max(best[j], __shfl_xor_sync(~0u, best[j], o));
-      const uint32_t h = HT >= 4 ? t * HEADS + j : HT == 2 ? t >> 1 : 0;
-      if (gl == 0) atomicMax(&s_max[h], best[j]);
-    }
-  }
-  __syncthreads();
-  if (tid < hn) a.chunk_max[(row0 + tid) * a.chunks + chunk] = s_max[tid];
 }
 
-// ---- exp -----------------------------------------------------------------------------------------
-// exp_in, exp_out and the row's sum.  The table (4 MB for the layer prover's) lives in L2; a thread has four
-// columns under way, since what it waits for is a chain of three loads.
-constexpr int EX_THREADS = 256, EX_COLS = 4;
-constexpr uint32_t EX_KEYS = EX_THREADS * EX_COLS;  // columns of a block
+// ---- softmax -------------------------------------------------------------------------------------------
+// exp_in, exp_out, the row's sum and the softmax of one row, by a cluster of up to 8 blocks that share their sums
+// through distributed shared memory: no pass over the scores for the sum alone.  The table (4 MB for the layer
+// prover's) lives in L2; a thread has four columns under way, since what it waits for is a chain of loads.
+constexpr uint32_t EX_COLS = 4, EX_MAX_THREADS = 1024;
 
-__global__ void __launch_bounds__(EX_THREADS) k_kv_exp(AttendArgs a) {
-  __shared__ int32_t s_max[EX_THREADS / 32];
-  __shared__ int64_t s_sum[EX_THREADS / 32];
+// A warp takes 128 columns at a time, a lane four that lie together where the rows of the witness begin on 16 bytes
+// (ALIGNED: one access each), else every 32nd.
+template <bool ALIGNED>
+__global__ void __launch_bounds__(EX_MAX_THREADS, 2) k_kv_softmax(AttendArgs a, uint32_t blocks) {
+  __shared__ int64_t s_part[32];
+  __shared__ int64_t s_sum;
+  __shared__ uint64_t s_inverse;
+  namespace cg = cooperative_groups;
+  constexpr uint32_t STEP = ALIGNED ? 1 : 32;  // between a lane's columns
   const KvView& c = a.c;
-  const uint32_t chunk = blockIdx.x % a.exp_chunks, row = blockIdx.x / a.exp_chunks, h = row % a.heads, b = row / a.heads, g = h / a.group;
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t cols = columns(a, b, false), first = chunk * EX_KEYS + threadIdx.x;
-  if (chunk * EX_KEYS >= cols) return;
-  const uint64_t at = (uint64_t)row * a.max_keys + first;
-  const unsigned char* valid = a.valid + ((uint64_t)b * c.kv_heads + g) * a.valid_stride + first;
-  bool in[EX_COLS];
-  int32_t s[EX_COLS];
+  const uint32_t rank = blockIdx.x % blocks, row = blockIdx.x / blocks, h = row % a.heads, b = row / a.heads, g = h / a.group;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, turn = blocks * blockDim.x * EX_COLS;
+  const uint32_t cols = columns(a, length(a, b, false));
+  if (cols == 0) return;
+  const uint32_t first = (rank * warps + warp) * 128 + lane * (ALIGNED ? 4 : 1), up = (cols + 31) & ~31u;
+  const uint64_t at = (uint64_t)row * a.max_keys;
+  const unsigned char* valid = a.valid + ((uint64_t)b * c.kv_heads + g) * a.padded;
+  auto which = [&](uint32_t i) {  // of the lane's four columns hold a position
+    uint32_t in = 0;
+    if (ALIGNED && i < up) {
+      const uchar4 v = *reinterpret_cast<const uchar4*>(valid + i);
+      in = v.x | v.y << 1 | v.z << 2 | v.w << 3;
+      if (i + 4 > cols) in &= i < cols ? (1u << (cols - i)) - 1 : 0;
+    }
 #pragma unroll
-  for (int j = 0; j < EX_COLS; j++) {
-    in[j] = first + j * EX_THREADS < cols && valid[j * EX_THREADS];
-    s[j] = first + j * EX_THREADS < cols ? a.score[at + j * EX_THREADS] : 0;
-  }
+    for (uint32_t j = 0; j < 4; j++)
+      if (!ALIGNED && i + j * STEP < cols && valid[i + j * STEP]) in |= 1u << j;
+    return in;
+  };
+  auto load = [&](const int32_t* from, uint32_t i, int32_t (&v)[4]) {
+    if (ALIGNED && i + 4 <= cols) {
+      const int4 x = *reinterpret_cast<const int4*>(from + at + i);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) v[j] = i + j * STEP < cols ? from[at + i + j * STEP] : 0;
+    }
+  };
+  auto store = [&](int32_t* to, uint32_t i, uint32_t in, const int32_t (&v)[4]) {
+    if (!to) return;
+    if (ALIGNED && in == 15) {
+      *reinterpret_cast<int4*>(to + at + i) = make_int4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++)
+        if (in >> j & 1) to[at + i + j * STEP] = v[j];
+    }
+  };
+
+  // the row's largest score: its pieces are those of the blocks whose spans it meets
+  const uint32_t rows = c.kv_heads * a.tiles, tile = h % a.group / a.score_heads, r = g * a.tiles + tile;
+  const uint32_t before = a.before[b], sets = (a.before[b + 1] - before) / rows, begin = before + r * sets;
+  const uint32_t span = (a.before[c.batch] + a.score_grid - 1) / a.score_grid, first_block = begin / span, last_block = (begin + sets - 1) / span;
   int32_t best = INT32_MIN;
-  const uint32_t used = (cols + a.chunk_keys - 1) / a.chunk_keys;
-  for (uint32_t i = threadIdx.x; i < used; i += EX_THREADS) best = max(best, a.chunk_max[(uint64_t)row * a.chunks + i]);
+  for (uint32_t i = first_block + lane; i <= last_block; i += 32)
+    best = max(best, a.piece_max[((uint64_t)b * rows + r + i) * a.score_heads + h % a.group % a.score_heads]);
   best = __reduce_max_sync(~0u, best);
-  if (lane == 0) s_max[warp] = best;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < EX_THREADS / 32; w++) best = max(best, s_max[w]);
+
   int64_t sum = 0;
   bool outside = false;
-  int32_t x[EX_COLS], e[EX_COLS];
+  for (uint32_t i = first; i < cols; i += turn) {
+    const uint32_t in = which(i);
+    int32_t s[4], e[4];
+    load(a.score, i, s);
 #pragma unroll
-  for (int j = 0; j < EX_COLS; j++) {
-    const int64_t d = in[j] ? (int64_t)s[j] - best : 0;
-    outside |= d < a.exp_low;
-    x[j] = (int32_t)max(d, (int64_t)a.exp_low);
-    e[j] = __ldg(a.exp + (x[j] - a.exp_low));
+    for (int j = 0; j < 4; j++) {
+      const int64_t d = in >> j & 1 ? (int64_t)s[j] - best : 0;
+      outside |= d < a.exp_low;
+      s[j] = (int32_t)max(d, (int64_t)a.exp_low);
+      e[j] = __ldg(a.exp + (s[j] - a.exp_low));
+    }
+    store(a.exp_in, i, in, s);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (!(in >> j & 1)) e[j] = 0;
+      if (e[j] < 0) { e[j] = 0; outside = true; }
+      sum += e[j];
+    }
+    store(a.exp_out, i, in, e);
   }
-#pragma unroll
-  for (int j = 0; j < EX_COLS; j++) {
-    if (!in[j]) continue;
-    if (e[j] < 0) { e[j] = 0; outside = true; }
-    sum += e[j];
-    if (a.exp_in) a.exp_in[at + j * EX_THREADS] = x[j];
-    a.exp_out[at + j * EX_THREADS] = e[j];
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  if (lane == 0) s_part[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    sum = lane < warps ? s_part[lane] : 0;
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (lane == 0) s_sum = sum;
+  }
+  // floor(top / sum) by the reciprocal floor((2^64 - 1) / sum): short by one at most.  The digits are written up to a
+  // multiple of 32 columns, zeros where a column holds no position.
+  if (blocks > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (threadIdx.x == 0) {
+      sum = 0;
+      for (uint32_t i = 0; i < blocks; i++) sum += *cluster.map_shared_rank(&s_sum, i);
+    }
+    cluster.sync();  // nobody's sum is overwritten or goes while another reads it
+  }
+  if (threadIdx.x == 0) {
+    s_sum = sum;
+    s_inverse = sum ? ~0ull / (uint64_t)sum : 0;
+    if (rank == 0) {
+      a.sum[row] = sum;
+      outside |= sum == 0;
+    }
   }
   if (outside) kv_flag(c, STATUS_KV_EXP);
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < EX_THREADS / 32; w++) sum += s_sum[w];
-    atomicAdd(reinterpret_cast<unsigned long long*>(a.sum + row), (unsigned long long)sum);
+  const uint64_t total = (uint64_t)s_sum, inverse = s_inverse;
+  unsigned char* const digits = a.digits + (uint64_t)row * 3 * a.padded;
+  int64_t weights = 0;
+  for (uint32_t i = first; i < up; i += turn) {
+    const uint32_t in = which(i);
+    int32_t o[4];
+    load(a.exp_out, i, o);  // this thread's own
+    uint32_t weight = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint64_t top = ((uint64_t)(uint32_t)o[j] << a.soft_shift) + total / 2, q = __umul64hi(top, inverse);
+      o[j] = in >> j & 1 && total ? (int32_t)((uint32_t)q + (top - q * total >= total ? 1u : 0u)) : 0;
+      weight += (uint32_t)o[j];
+    }
+    weights += weight;
+    store(a.softmax, i, in, o);
+#pragma unroll
+    for (int d = 0; d < 3; d++) {
+      unsigned char* to = digits + d * a.padded + i;
+      if (ALIGNED) {
+        *reinterpret_cast<uint32_t*>(to) = __byte_perm(__byte_perm(o[0], o[1], d | (4 + d) << 4), __byte_perm(o[2], o[3], d | (4 + d) << 4), 0x5410);
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+          if (i + j * STEP < up) to[j * STEP] = (unsigned char)(o[j] >> 8 * d);
+      }
+    }
   }
+  for (int o = 16; o; o >>= 1) weights += __shfl_xor_sync(~0u, weights, o);
+  if (lane == 0 && weights) atomicAdd(reinterpret_cast<unsigned long long*>(a.weight + row), (unsigned long long)weights);
 }
 
 // ---- values ----------------------------------------------------------------------------------------
 // sum_j o_j v_j exactly, on the same instruction.  o is at most 2^20: three unsigned digits base 256, which are
-// the operand columns (3 per head); the rows are the bytes of v (v' = v + bias unsigned), so that
+// operand columns; the rows are the bytes of v (v' = v + bias unsigned), so that
 //   sum_j o_j v_j = sum_p,r 256^(p + r) (byte plane p of v' . digit r of o) - bias sum_j o_j.
-// A warp takes 32 keys x 128 bytes of their rows: lane (g, t) loads 16 bytes of the 8 keys 8t .. 8t+7, and
-// turning 4 keys x 4 bytes in registers (8 byte permutes) gives the A registers, keys along the instruction's
-// inner dimension.  Sums of a chunk of at most 1024 keys stay far below 2^31.  The 8 bytes of digits that a lane
-// needs for 32 keys lie together in shared memory.
-// What bounds it: bytes of the values; 32 keys x 128 bytes cost a warp about 100 instructions of the 700 that
-// an SM quarter issues while they arrive.
-constexpr uint32_t VA_CHUNK = 1024;           // keys of a block at most
-constexpr uint32_t VA_STRIDE = VA_CHUNK + 32; // bytes of a column's digits: eight columns on different banks
-__host__ __device__ constexpr int va_tiles(int ht) { return (3 * ht + 7) / 8; }                   // instruction columns in eights
-__host__ __device__ constexpr int va_threads(int ht) { return va_tiles(ht) > 2 ? 128 : 256; }     // by the registers of the sums
-constexpr int VA_STAGES = 2;
-constexpr size_t va_smem(int ht) {  // queues (later partial sums of 8 columns), digits, places of the keys
-  return (size_t)va_threads(ht) / 32 * VA_STAGES * 4096 + (size_t)VA_STRIDE * 8 * va_tiles(ht) + VA_CHUNK * 8;
-}
+// Sums of a block's keys stay below 2^31 (see VA_SETS).
+// A warp takes 128 bytes of 32 rows for 4 heads (or for the 1 or 2 that there are): lane (g, t) has 16 bytes of the
+// rows 8 t .. 8 t + 7, and turning 4 keys x 4 bytes in registers (8 byte permutes) gives the A registers, keys
+// along the instruction's inner dimension; the 8 bytes of a column's digits are a lane's B registers as they
+// lie.  The three digits of a head are columns of one lane (one pair of lanes with fewer than 4 heads), so a
+// warp adds its heads' sums to the output without meeting another warp.
+// What bounds it: bytes of the values; 32 keys x 128 bytes cost a warp about 160 instructions of the 700 that an
+// SM quarter issues while they arrive.
+constexpr uint32_t VA_SETS = 512;  // sets of 32 keys whose products a register takes: 16384 x 255 x 255 < 2^31
+constexpr int VA_THREADS = 256, VA_WARPS = VA_THREADS / 32, VA_STAGES = 3;
+constexpr uint32_t VA_STEP = 4096 + 512;   // bytes of a step: 32 rows x 128 bytes, and digits
 
 // bytes [key][plane] of 4 words -> words [plane] of 4 keys
 __device__ __forceinline__ void turn4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&o)[4]) {
@@ -432,204 +592,211 @@ __device__ __forceinline__ void turn4(uint32_t a, uint32_t b, uint32_t c, uint32
   o[3] = __byte_perm(ab1, cd1, 0x7632);
 }
 
-template <int EB, int HT>
-__global__ void __launch_bounds__(va_threads(HT), 512 / va_threads(HT) - (va_tiles(HT) > 2 ? 1 : 0)) k_kv_values(AttendArgs a) {
-  constexpr int NT = va_tiles(HT), THREADS = va_threads(HT);
-  constexpr uint32_t ELEMS = 128 / EB;       // channels of a warp
-  extern __shared__ uint4 s_dyn[];
-  __shared__ unsigned long long s_total[HT];
-  __shared__ int64_t s_sum[HT];
-  __shared__ double s_inverse[HT];
-  __shared__ uint32_t s_last;
-  unsigned char* const s_digits = reinterpret_cast<unsigned char*>(s_dyn + THREADS / 32 * VA_STAGES * 256);
-  int64_t* const s_at = reinterpret_cast<int64_t*>(s_digits + VA_STRIDE * 8 * NT);
+// NH: heads of a warp, 1, 2 or 4.  A block takes a.v_heads = NH or 8.
+template <int EB, int NH>
+__global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
+  constexpr int NT = NH == 4 ? 2 : 1;      // columns of a warp in eights
+  constexpr uint32_t ELEMS = 128 / EB;     // channels of a warp
+  extern __shared__ uint4 s_dyn[];         // the lanes' queues
+  __shared__ uint32_t s_before[AT_BATCH + 1];
   const KvView& c = a.c;
   const uint32_t D = c.head_dim, row_bytes = D * EB, segments = (row_bytes + 127) / 128;
-  uint32_t x = blockIdx.x;
-  const uint32_t tile = x % a.v_tiles;
-  x /= a.v_tiles;
-  const uint32_t part = x % a.v_parts;
-  x /= a.v_parts;
-  const uint32_t chunk = x % a.v_chunks, row = x / a.v_chunks, g = row % c.kv_heads, b = row / c.kv_heads;
-  const uint32_t h0 = g * a.group + tile * HT, hn = min((uint32_t)HT, a.group - tile * HT);
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t = lane & 3;
-  const uint32_t n = kv_length(c, a.len, b, a.selected ? ~0ull : a.max_keys, false), cols = columns(a, b, false);
-  const uint32_t first = chunk * a.v_chunk_keys, keys = min(cols, first + a.v_chunk_keys) - first;
-  if (first >= cols) return;
-  const uint64_t row0 = (uint64_t)b * a.heads + h0;
-  const uint32_t wd = warp % a.v_split, wk = warp / a.v_split, groups = THREADS / 32 / a.v_split;
-  const uint32_t segment = part * a.v_split + wd, byte = segment * 128 + gl * 16;
-  const bool in_row = segment < segments && byte < row_bytes;
-  const uint32_t padded = (keys + 31) & ~31u;
-  for (uint32_t j = tid; j < padded; j += THREADS) {
-    uint32_t slot = 0;
-    const int32_t page = j < keys ? column_page(a, b, g, n, first + j, slot, false) : -1;
-    s_at[j] = page >= 0 ? page * c.page_stride + g * c.head_stride + slot * c.slot_stride : -1;
-  }
-  if (tid < HT) {
-    s_total[tid] = 0;
-    s_sum[tid] = tid < hn ? a.sum[row0 + tid] : 0;
-    s_inverse[tid] = s_sum[tid] > 0 ? 1.0 / (double)s_sum[tid] : 0.0;
-  }
-  __syncthreads();
+  const uint32_t rows = c.kv_heads * a.v_parts * a.v_tiles, members = a.v_split * (a.v_heads / NH), teams = VA_WARPS / members;
+  const uint32_t team = warp / members, member = warp % members, seg = member % a.v_split, hg = member / a.v_split;
+  const uint32_t total = plan_sets(a, s_before, 32, rows, false);
+  const uint32_t span = (total + gridDim.x - 1) / gridDim.x;
+  const uint32_t begin = min(total, blockIdx.x * span), end = min(total, begin + span);
 
-  uint4* const queue = s_dyn + (uint64_t)warp * VA_STAGES * 256 + lane;
-  auto fetch = [&](uint32_t k0, uint32_t stage) {
-    if (k0 < padded) {
+  // what a row of the plan is to this warp: its heads and its segment; hn 0: nothing
+  auto place_of = [&](uint32_t row, uint32_t& g, uint32_t& h0, uint32_t& segment) {
+    const uint32_t tile = row % a.v_tiles, part = row / a.v_tiles % a.v_parts, in_tile = min(a.v_heads, a.group - tile * a.v_heads);
+    g = row / a.v_tiles / a.v_parts;
+    h0 = g * a.group + tile * a.v_heads + hg * NH;
+    segment = part * a.v_split + seg;
+    return in_tile > hg * NH && segment < segments ? min((uint32_t)NH, in_tile - hg * NH) : 0u;
+  };
+  // the column that this lane brings for: head and digit; with four heads, digit 2 of the even ones in the second eight
+  const uint32_t col_head = NH == 4 ? gl / 2 : gl / 4, col_digit = NH == 4 ? gl % 2 : gl % 4;
+
+  // `fetch` walks the warp's sets VA_STAGES - 1 ahead of their use, and where their rows lie one more.  A lane's place in
+  // a step: the 128 bytes of a row side by side (they arrive together), their order turned with t so that the lanes
+  // that read together meet different banks; behind the rows the digits, 8 bytes a lane and eight of columns.
+  char* const queue = reinterpret_cast<char*>(s_dyn) + warp * VA_STAGES * VA_STEP;
+  const uint32_t my_rows = (t * 8 + (gl ^ (2 * t))) * 16, my_digits = 4096 + lane * 8;
+  const bool in_page = c.page_size % 8 == 0;  // then the rows 8 t .. 8 t + 7 lie one slot apart
+  uint32_t ahead_at = begin, ahead_left = 0, ahead_stage = 0;
+  bool ahead_has = false, ahead_in = false;
+  const char* ahead_base = nullptr;
+  const int64_t* ahead_rows = nullptr;
+  const unsigned char* ahead_digits = nullptr;
+  int64_t next_row = 0;
+  auto settle = [&]() {  // on to the piece that holds the warp's next set, if its sets of this one are over
+    while (ahead_left == 0 && ahead_at < end) {
+      const Piece p = piece_at(a, s_before, rows, ahead_at, end);
+      uint32_t g, h0, segment;
+      const uint32_t hn = place_of(p.row, g, h0, segment);
+      ahead_at += p.count;
+      if (!hn || p.count <= team) continue;
+      ahead_left = (p.count - team + teams - 1) / teams;
+      ahead_in = segment * 128 + gl * 16 < row_bytes;
+      ahead_base = c.v + segment * 128 + gl * 16;
+      ahead_has = col_head < hn && col_digit < 3;
+      const uint64_t key0 = (uint64_t)(p.first_set + team) * 32;
+      ahead_rows = a.row_at + ((uint64_t)p.b * c.kv_heads + g) * a.padded + key0 + (in_page ? 8 * t : lane);
+      ahead_digits = a.digits + (((uint64_t)p.b * a.heads + h0 + (ahead_has ? col_head : 0)) * 3 + (ahead_has ? col_digit : 0)) * a.padded + key0 + 8 * t;
+      next_row = *ahead_rows;
+    }
+  };
+  settle();
+  auto fetch = [&]() {
+    if (ahead_left) {
+      char* const to = queue + ahead_stage * VA_STEP;
+      const char* from = ahead_base + next_row;
+      if (in_page) {
+        if (ahead_in) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int64_t at = s_at[k0 + 8 * t + j];
-        const bool there = in_row && at >= 0;
-        copy_async(queue + (stage * 8 + j) * 32, there ? c.v + at + byte : c.v, there);
+          for (int j = 0; j < 8; j++) {
+            copy_async(to + my_rows + j * 512, from);
+            from += c.slot_stride;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const int64_t row = __shfl_sync(~0u, next_row, 8 * t + j);
+          if (ahead_in) copy_async(to + my_rows + j * 512, ahead_base + row);
+        }
       }
+      if (ahead_has) {
+        copy_async_8(to + my_digits, ahead_digits);
+        if (NT == 2 && col_digit == 0) copy_async_8(to + my_digits + 256, ahead_digits + 2 * a.padded);
+      }
+      ahead_stage = ahead_stage + 1 == VA_STAGES ? 0 : ahead_stage + 1;
+      ahead_rows += teams * 32;
+      ahead_digits += teams * 32;
+      if (--ahead_left) next_row = *ahead_rows;
+      else settle();
     }
     copy_commit();
   };
-  fetch(wk * 32, 0);
-  fetch((wk + groups) * 32, 1);
-
-  // the softmax of the chunk, while the first values are under way
-  for (uint32_t j = tid; j < padded; j += THREADS) {
-    const bool there = s_at[j] >= 0;
-    int32_t e[HT];
-#pragma unroll
-    for (int h = 0; h < HT; h++) e[h] = there && h < hn ? a.exp_out[(row0 + h) * a.max_keys + first + j] : 0;
-#pragma unroll
-    for (int h = 0; h < HT; h++) {
-      uint32_t o = 0;
-      if (there && h < hn) {
-        const int64_t sum = s_sum[h], top = ((int64_t)e[h] << a.soft_shift) + sum / 2;
-        if (sum > 0) {
-          // the quotient is at most 2^20: a 64-bit floating point estimate is off by one at most
-          int64_t k = (int64_t)((double)top * s_inverse[h]);
-          const int64_t r = top - k * sum;
-          k += r < 0 ? -1 : r >= sum ? 1 : 0;
-          o = (uint32_t)k;
-        }
-        if (a.softmax && part == 0) a.softmax[(row0 + h) * a.max_keys + first + j] = (int32_t)o;
-      }
-      s_digits[(3 * h) * VA_STRIDE + j] = (unsigned char)o;
-      s_digits[(3 * h + 1) * VA_STRIDE + j] = (unsigned char)(o >> 8);
-      s_digits[(3 * h + 2) * VA_STRIDE + j] = (unsigned char)(o >> 16);
-      const uint32_t warp_sum = __reduce_add_sync(~0u, o);  // at most 32 x 2^20; whole warps: padded is a multiple of 32
-      if (lane == 0 && warp_sum) atomicAdd(&s_total[h], (unsigned long long)warp_sum);
-    }
-#pragma unroll
-    for (int k = 3 * HT; k < 8 * NT; k++) s_digits[k * VA_STRIDE + j] = 0;
-  }
-  __syncthreads();
-
-  int32_t acc[8][NT][4];
-#pragma unroll
-  for (int m = 0; m < 8; m++)
-#pragma unroll
-    for (int k = 0; k < NT; k++) acc[m][k][0] = acc[m][k][1] = acc[m][k][2] = acc[m][k][3] = 0;
-  uint32_t stage = 0;
 #pragma unroll 1
-  for (uint32_t k0 = wk * 32; k0 < padded; k0 += groups * 32) {
-    copy_wait<VA_STAGES - 1>();
-    uint4 v[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = queue[(stage * 8 + j) * 32];
-    uint2 d[NT];
-#pragma unroll
-    for (int k = 0; k < NT; k++) d[k] = *reinterpret_cast<const uint2*>(s_digits + (k * 8 + gl) * VA_STRIDE + k0 + 8 * t);
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-      uint32_t p[4], r[4];
-      auto word = [&](int j) { return w == 0 ? v[j].x : w == 1 ? v[j].y : w == 2 ? v[j].z : v[j].w; };
-      turn4(word(0), word(1), word(2), word(3), p);
-      turn4(word(4), word(5), word(6), word(7), r);
-      p[3] ^= 0x80808080u;
-      r[3] ^= 0x80808080u;
-      if (EB == 2) { p[1] ^= 0x80808080u; r[1] ^= 0x80808080u; }
-#pragma unroll
-      for (int k = 0; k < NT; k++) {
-        mma_u8u8(acc[2 * w][k], p[0], p[1], r[0], r[1], d[k].x, d[k].y);
-        mma_u8u8(acc[2 * w + 1][k], p[2], p[3], r[2], r[3], d[k].x, d[k].y);
-      }
-    }
-    fetch(k0 + 2 * groups * 32, stage);  // every register of this place has been used
-    stage ^= 1;
-  }
-  copy_wait<0>();
+  for (int i = 0; i < VA_STAGES - 1; i++) fetch();
 
-  // weights of the byte planes in the lane; digits and the warps that dealt the keys through shared memory:
-  // s_part[warp][column of eight][channel], eight columns at a time
-  int64_t* s_part = reinterpret_cast<int64_t*>(s_dyn);
-  const uint32_t outputs = a.v_split * ELEMS;  // channels of the block
-  constexpr int MINE = (HT * THREADS / 32 * ELEMS + THREADS - 1) / THREADS;  // (head, channel) of a thread at most
-  uint64_t mine[MINE];
+  uint32_t stage = 0;
+  bool range = false;
+  for (uint32_t at = begin; at < end;) {
+    const uint32_t here = at;
+    uint32_t count;
+    {
+      const Piece p = piece_at(a, s_before, rows, at, end);
+      uint32_t g, h0, segment;
+      count = p.count;
+      at += count;
+      if (!place_of(p.row, g, h0, segment) || count <= team) continue;
+    }
+    int32_t acc[8][NT][4];
 #pragma unroll
-  for (int i = 0; i < MINE; i++) mine[i] = 0;
+    for (int k = 0; k < NT; k++)
 #pragma unroll
-  for (int k = 0; k < NT; k++) {
-    __syncthreads();
+      for (int m = 0; m < 8; m++) acc[m][k][0] = acc[m][k][1] = acc[m][k][2] = acc[m][k][3] = 0;
+#pragma unroll 1
+    for (uint32_t k = team; k < count; k += teams) {
+      copy_wait<VA_STAGES - 2>();
+      const char* const step = queue + stage * VA_STEP;
+      stage = stage + 1 == VA_STAGES ? 0 : stage + 1;
+      fetch();  // into the place that was read a step ago
+      uint2 d[NT];
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+      for (int z = 0; z < NT; z++) d[z] = *reinterpret_cast<const uint2*>(step + my_digits + z * 256);
+      // 8 bytes of the rows at a time: all 16 together would not leave registers for two blocks an SM
 #pragma unroll
       for (int half = 0; half < 2; half++) {
-        const uint64_t a0 = (uint64_t)(int64_t)acc[2 * w][k][half] + ((uint64_t)(int64_t)acc[2 * w][k][2 + half] << 8);
-        const uint64_t a1 = (uint64_t)(int64_t)acc[2 * w + 1][k][half] + ((uint64_t)(int64_t)acc[2 * w + 1][k][2 + half] << 8);
-        int64_t* to = s_part + ((uint64_t)warp * 8 + 2 * t + half) * ELEMS;
-        if (EB == 4) {
-          to[gl * 4 + w] = (int64_t)(a0 + (a1 << 16));
-        } else {
-          to[gl * 8 + 2 * w] = (int64_t)a0;
-          to[gl * 8 + 2 * w + 1] = (int64_t)a1;
+        uint2 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = *reinterpret_cast<const uint2*>(step + my_rows + j * 512 + half * 8);
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+          const int w = 2 * half + z;
+          uint32_t lo[4], hi[4];
+          auto word = [&](int j) { return z == 0 ? v[j].x : v[j].y; };
+          turn4(word(0), word(1), word(2), word(3), lo);
+          turn4(word(4), word(5), word(6), word(7), hi);
+          lo[3] ^= 0x80808080u;
+          hi[3] ^= 0x80808080u;
+          if (EB == 2) { lo[1] ^= 0x80808080u; hi[1] ^= 0x80808080u; }
+#pragma unroll
+          for (int k = 0; k < NT; k++) {
+            mma_u8u8(acc[2 * w][k], lo[0], lo[1], hi[0], hi[1], d[k].x, d[k].y);
+            mma_u8u8(acc[2 * w + 1][k], lo[2], lo[3], hi[2], hi[3], d[k].x, d[k].y);
+          }
         }
       }
     }
-    __syncthreads();
+    const Piece p = piece_at(a, s_before, rows, here, end);
+    uint32_t g, h0, segment;
+    const uint32_t hn = place_of(p.row, g, h0, segment);
+    // how many sums come together in the row's output: of each of its pieces, the teams that have a set of it
+    const uint32_t start = min(p.sets, span - p.begin % span), others = p.sets - start;
+    const uint32_t adders = min(teams, start) + others / span * min(teams, span) + min(teams, others % span);
+    // Lane (g, t): columns 2t and 2t + 1 of each eight.  With four heads both digits 0 and 1 of head t lie there and
+    // digit 2 in the second eight; with one or two, digit 2 lies in the next lane.
+    const uint32_t head = NH == 4 ? t : t / 2, channel = segment * ELEMS + gl * (16 / EB);
+    const bool mine = head < hn && (NH == 4 || t % 2 == 0);
+    constexpr uint64_t BIAS = EB == 4 ? uint64_t(1) << 31 : uint64_t(1) << 15;
+    auto join = [&](uint64_t c0, uint64_t c1, uint64_t c2) {
+      if (NH != 4) c2 = __shfl_xor_sync(~0u, c0, 1);
+      return c0 + (c1 << 8) + (c2 << 16);
+    };
+    const uint64_t row = (uint64_t)p.b * a.heads + h0 + (mine ? head : 0), to = row * D + channel;
+    const uint64_t below = BIAS * (uint64_t)a.weight[row];
+    auto finish = [&](uint64_t biased, uint64_t where) {
+      const int64_t sum = (int64_t)(biased - below), y = rdiv(sum, a.soft_shift);
+      a.out[where] = saturate(y, INT32_MIN, INT32_MAX, range);
+      if (a.out_rem) a.out_rem[where] = (int32_t)(uint32_t)((uint64_t)sum - ((uint64_t)y << a.soft_shift));
+    };
 #pragma unroll
-    for (int i = 0; i < MINE; i++) {
-      const uint32_t at = i * THREADS + tid, h = at / outputs, ch = at % outputs;
-      if (h < hn) {
-        for (uint32_t r = 0; r < 3; r++) {
-          const uint32_t col = 3 * h + r;
-          if (col / 8 != k) continue;
-          uint64_t v = 0;
-          for (uint32_t z = 0; z < groups; z++)
-            v += (uint64_t)s_part[((uint64_t)(z * a.v_split + ch / ELEMS) * 8 + col % 8) * ELEMS + ch % ELEMS];
-          mine[i] += v << (8 * r);
+    for (int w = 0; w < 4; w++) {
+      uint64_t plane[3][2];  // digit columns: bytes 0 and 1, bytes 2 and 3 of the word
+#pragma unroll
+      for (int z = 0; z < 3; z++) {
+        const int k = z == 2 ? NT - 1 : 0, half = z == 1 ? 1 : 0;
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+          plane[z][m] = (uint64_t)(int64_t)acc[2 * w + m][k][half] + ((uint64_t)(int64_t)acc[2 * w + m][k][2 + half] << 8);
+      }
+      uint64_t value[4 / EB];
+      if (EB == 4) {
+        value[0] = join(plane[0][0] + (plane[0][1] << 16), plane[1][0] + (plane[1][1] << 16), plane[2][0] + (plane[2][1] << 16));
+      } else {
+#pragma unroll
+        for (int m = 0; m < 4 / EB; m++) value[m] = join(plane[0][m % 2], plane[1][m % 2], plane[2][m % 2]);
+      }
+#pragma unroll
+      for (int m = 0; m < 4 / EB; m++) {
+        const uint32_t e = w * (4 / EB) + m;
+        if (mine && channel + e < D) {
+          if (adders == 1) finish(value[m], to + e);
+          else atomicAdd(reinterpret_cast<unsigned long long*>(a.acc + to + e), (unsigned long long)value[m]);
         }
       }
     }
-  }
-  const uint64_t bias = EB == 4 ? uint64_t(1) << 31 : uint64_t(1) << 15;
-  const uint32_t used = (cols + a.v_chunk_keys - 1) / a.v_chunk_keys;
-  const uint32_t ch0 = part * outputs;
-  bool range = false;
-  auto finish = [&](int64_t sum, uint64_t at) {
-    const int64_t y = rdiv(sum, a.soft_shift);
-    a.out[at] = saturate(y, INT32_MIN, INT32_MAX, range);
-    if (a.out_rem) a.out_rem[at] = (int32_t)(uint32_t)((uint64_t)sum - ((uint64_t)y << a.soft_shift));
-  };
-#pragma unroll
-  for (int i = 0; i < MINE; i++) {
-    const uint32_t at = i * THREADS + tid, h = at / outputs, ch = ch0 + at % outputs;
-    if (h < hn && ch < D) {
-      const uint64_t v = mine[i] - bias * (uint64_t)s_total[h], to = (row0 + h) * D + ch;
-      if (used == 1) finish((int64_t)v, to);
-      else atomicAdd(reinterpret_cast<unsigned long long*>(a.acc + to), (unsigned long long)v);
-    }
-  }
-  if (used > 1) {
-    // the last of the row's blocks brings the sums to the output
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) s_last = atomicAdd(a.done + (((uint64_t)row * a.v_tiles + tile) * a.v_parts + part), 1u) == used - 1;
-    __syncthreads();
-    if (s_last) {
+    if (adders > 1) {
+      // the last of the warps that add to these channels brings the sums to the output
       __threadfence();
-      for (uint32_t at = tid; at < hn * outputs; at += THREADS) {
-        const uint32_t h = at / outputs, ch = ch0 + at % outputs;
-        if (ch < D) finish(__ldcg(a.acc + (row0 + h) * D + ch), (row0 + h) * D + ch);
+      __syncwarp();
+      uint32_t nth = 0;
+      if (lane == 0) nth = atomicAdd(a.done + ((uint64_t)p.b * rows + p.row) * VA_WARPS + member, 1u);
+      nth = __shfl_sync(~0u, nth, 0);
+      if (nth == adders - 1) {
+        __threadfence();
+        for (uint32_t e = 0; e < 16 / EB; e++)
+          if (mine && channel + e < D) finish((uint64_t)__ldcg(reinterpret_cast<const long long*>(a.acc) + to + e), to + e);
       }
     }
   }
+  copy_wait<0>();
   if (range) kv_flag(c, STATUS_KV_RANGE);
-  if (chunk == 0 && part == 0 && tid < hn && a.sum[row0 + tid] == 0) kv_flag(c, STATUS_KV_EXP);
 }
 
 template <class K>
@@ -641,88 +808,109 @@ static int launch(grape_ctx* ctx, K kernel, const AttendArgs& a, uint64_t grid, 
 }
 
 template <int EB>
-static int launch_scores(grape_ctx* ctx, const AttendArgs& a, uint32_t ht, uint64_t grid, uint32_t threads, size_t smem) {
-  return launch(ctx, ht == 1 ? k_kv_scores<EB, 1> : ht == 2 ? k_kv_scores<EB, 2> : ht == 4 ? k_kv_scores<EB, 4> : k_kv_scores<EB, 8>, a, grid, threads,
-                smem);
+static int launch_scores(grape_ctx* ctx, const AttendArgs& a, uint32_t threads, size_t smem) {
+  const uint32_t h = a.score_heads;
+  auto kernel = a.score_keys == 32 ? (h == 1 ? k_kv_scores<EB, 1, 2> : h == 2 ? k_kv_scores<EB, 2, 2> : k_kv_scores<EB, 4, 2>)
+                                   : (h == 1 ? k_kv_scores<EB, 1, 1> : h == 2 ? k_kv_scores<EB, 2, 1> : k_kv_scores<EB, 4, 1>);
+  return launch(ctx, kernel, a, a.score_grid, threads, smem);
+}
+
+static int launch_softmax(grape_ctx* ctx, const AttendArgs& a, uint64_t rows, uint64_t cols) {
+  // A thread has its four columns once where the GPU holds that many threads; with more rows than that it takes
+  // turns.  Threads of a block first, up to 1024, then blocks of a cluster, up to 8.
+  const uint64_t room = (uint64_t)ctx->sm_count * 2048 * 2;
+  uint32_t blocks = 1, threads = 256;
+  while (threads < EX_MAX_THREADS && (uint64_t)threads * EX_COLS < cols && rows * threads * 2 <= room) threads *= 2;
+  while (blocks < 8 && (uint64_t)blocks * threads * EX_COLS < cols && rows * blocks * threads * 2 <= room) blocks *= 2;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = blocks;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((uint32_t)(rows * blocks));
+  config.blockDim = dim3(threads);
+  config.stream = ctx->stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  GRAPE_CUDA_TRY(ctx, cudaLaunchKernelEx(&config, a.max_keys % 4 ? k_kv_softmax<false> : k_kv_softmax<true>, a, blocks));
+  ctx->launches += 1;
+  return GRAPE_OK;
 }
 
 template <int EB>
-static int launch_values(grape_ctx* ctx, const AttendArgs& a, uint32_t ht, uint64_t grid) {
-  return launch(ctx, ht == 1 ? k_kv_values<EB, 1> : ht == 2 ? k_kv_values<EB, 2> : ht == 5 ? k_kv_values<EB, 5> : k_kv_values<EB, 8>, a, grid,
-                va_threads(ht), va_smem(ht));
+static int launch_values(grape_ctx* ctx, const AttendArgs& a, uint64_t grid) {
+  const uint32_t h = a.v_heads;
+  return launch(ctx, h == 1 ? k_kv_values<EB, 1> : h == 2 ? k_kv_values<EB, 2> : k_kv_values<EB, 4>, a, grid, VA_THREADS, VA_WARPS * VA_STAGES * VA_STEP);
 }
 
-static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs& a) {
+static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs a) {
   const uint64_t rows = (uint64_t)a.c.batch * a.heads, D = cache->head_dim, kv_rows = (uint64_t)a.c.batch * cache->kv_heads;
   const uint64_t all = a.selected ? (uint64_t)a.n_select * cache->page_size : (uint64_t)a.c.width * cache->page_size;
   const uint64_t cols = std::min(all, a.max_keys);
-  const uint32_t row_bytes = (uint32_t)(D * cache->bits / 8), sms = (uint32_t)ctx->sm_count;
+  const uint32_t row_bytes = (uint32_t)(D * cache->bits / 8), blks = (row_bytes + 63) / 64, sms = (uint32_t)ctx->sm_count;
 
-  // Scores: heads of a block (their columns are 8 times a key's bytes), warps that share a row of long keys
-  // (eight 64-byte steps each at least), and keys of a block: 256 KB of them, fewer while that leaves the GPU
-  // with under four blocks an SM.
-  uint32_t ht = 1;
-  while (ht < 8 && ht < a.group && (uint64_t)2 * ht * row_bytes * 8 <= SC_SMEM) ht *= 2;
-  a.tiles = (a.group + ht - 1) / ht;
-  const uint32_t blks = (row_bytes + 63) / 64, mt = sc_sixteens(ht);
-  const size_t columns_bytes = (size_t)blks * ht * 512, queue_bytes = (size_t)sc_stages(ht) * mt * 1024, part_bytes = (size_t)2 * mt * ht * 64;
-  // columns that leave room for one block an SM: 16 warps instead of 8, where their queues still fit
-  const uint32_t threads = columns_bytes >= 48 * 1024 && columns_bytes + 16 * (queue_bytes + part_bytes) <= SC_SMEM_ALL ? 512 : 256;
+  // Scores.  Rows up to 1 KB: two blocks of 8 warps an SM, a warp a set of 32 keys.  Longer ones: one block of 16
+  // warps, 16 keys at a time, a row shared by as many warps as have 8 blocks of it (a few rows of a long head are
+  // few sets).  Heads of a tile: as many as there are up to 4, while their columns fit.
+  const int mt = row_bytes <= 1024 ? 2 : 1;
+  const uint32_t threads = mt == 2 ? 256 : 512, warps = threads / 32;
+  a.score_keys = 16 * mt;
   a.split = 1;
-  while (a.split < threads / 32 && blks / (2 * a.split) >= 8) a.split *= 2;
-  const size_t smem = columns_bytes + threads / 32 * (queue_bytes + (a.split > 1 ? part_bytes : 0));
-  const uint32_t step = threads / 32 / a.split * 16 * mt;
-  uint64_t keys = std::max<uint64_t>(step, (256 * 1024 / row_bytes + step - 1) / step * step);
-  while (keys > step && kv_rows * a.tiles * ((cols + keys - 1) / keys) < 4ull * sms) keys = std::max<uint64_t>(step, keys / 2 / step * step);
-  a.chunk_keys = (uint32_t)keys;
-  const uint64_t chunks = (cols + keys - 1) / keys, exp_chunks = (cols + EX_KEYS - 1) / EX_KEYS;
+  while (mt == 1 && a.split < warps && blks / (2 * a.split) >= 8) a.split *= 2;
+  const size_t room = (mt == 2 ? AT_SMEM : AT_SMEM_ALONE) - warps * sc_warp(mt);
+  uint32_t ht = 1;
+  while (ht < 4 && ht < a.group && (size_t)2 * ht * blks * 512 <= room) ht *= 2;
+  a.score_heads = ht;
+  a.tiles = (a.group + ht - 1) / ht;
+  const size_t smem = (size_t)blks * ht * 512 + warps * sc_warp(mt);
+  const uint64_t sets = kv_rows * a.tiles * ((cols + a.score_keys - 1) / a.score_keys);
+  a.score_grid = (uint32_t)std::min<uint64_t>((mt == 2 ? 2 : 1) * sms, sets);
 
-  // Values: heads of a block (three columns each, in eights), 128-byte segments of a row dealt to the warps,
-  // the rest of the warps share the keys.
-  const uint32_t v_ht = a.group == 1 ? 1 : a.group == 2 ? 2 : a.group <= 5 ? 5 : 8;
-  a.v_tiles = (a.group + v_ht - 1) / v_ht;
-  const uint32_t segments = (row_bytes + 127) / 128, v_warps = va_threads(v_ht) / 32;
+  // Values: 4 heads a warp, 8 a block where a key head has more than 4 and the segments of a row leave warps for
+  // it; up to 8 segments of 128 bytes a block, the rest of a row in other parts; teams share the keys.
+  const uint32_t segments = (row_bytes + 127) / 128;
   a.v_split = 1;
-  while (a.v_split < v_warps && a.v_split < segments) a.v_split *= 2;
+  while (a.v_split < VA_WARPS && a.v_split < segments) a.v_split *= 2;
+  a.v_heads = a.group == 1 ? 1 : a.group == 2 ? 2 : a.group <= 4 || a.v_split == VA_WARPS ? 4 : 8;
+  a.v_tiles = (a.group + a.v_heads - 1) / a.v_heads;
   a.v_parts = (segments + a.v_split - 1) / a.v_split;
-  const uint32_t v_step = v_warps / a.v_split * 32;
-  uint64_t v_keys = VA_CHUNK;
-  while (v_keys > v_step && kv_rows * a.v_tiles * a.v_parts * ((cols + v_keys - 1) / v_keys) < 4ull * sms) v_keys /= 2;
-  a.v_chunk_keys = (uint32_t)v_keys;
-  const uint64_t v_chunks = (cols + v_keys - 1) / v_keys;
+  const uint64_t v_rows = kv_rows * a.v_parts * a.v_tiles, v_sets = v_rows * ((cols + 31) / 32);
+  // a block's span of sets bounds the sums of a register
+  const uint64_t v_grid = std::max<uint64_t>(std::min<uint64_t>(2 * sms, v_sets), (v_sets + VA_SETS - 1) / VA_SETS);
 
   const uint64_t most = 0x7fffffffu;
-  if (kv_rows * a.tiles * chunks > most || rows * exp_chunks > most || kv_rows * a.v_tiles * a.v_parts * v_chunks > most ||
-      rows * D > (uint64_t(1) << 38))
+  if (sets > most || rows > most || v_sets > most || rows * D > (uint64_t(1) << 38))
     return kv_refuse(ctx, GRAPE_ERR_LIMIT, "too many rows and columns for one call");
-  a.chunks = (uint32_t)chunks;
-  a.exp_chunks = (uint32_t)exp_chunks;
-  a.v_chunks = (uint32_t)v_chunks;
-  const uint64_t dones = kv_rows * a.v_tiles * a.v_parts;
-  a.done_per_row = (uint32_t)((uint64_t)a.v_tiles * a.v_parts);
-  a.valid_stride = (cols + 15) & ~uint64_t(15);
+  a.acc_count = rows * D;
+  a.done_count = v_rows * VA_WARPS;
+  a.padded = (cols + 31) & ~uint64_t(31);
   auto up = [](uint64_t n) { return (n + 255) & ~uint64_t(255); };
-  const uint64_t b_max = up(rows * chunks * 4), b_acc = up(rows * D * 8), b_done = up(dones * 4), b_valid = up(kv_rows * a.valid_stride), b_sum = a.sum ? 0 : up(rows * 8);
+  const uint64_t b_max = up((kv_rows * a.tiles + a.score_grid) * ht * 4), b_before = up((a.c.batch + 1) * 4), b_acc = up(a.acc_count * 8);
+  const uint64_t b_done = up(a.done_count * 4), b_valid = up(kv_rows * a.padded), b_digits = up(rows * 3 * a.padded), b_rows = up(kv_rows * a.padded * 8), b_weight = up(rows * 8), b_sum = a.sum ? 0 : up(rows * 8);
   const uint64_t b_keys = up(rows * a.max_keys * 4);
   void* w = nullptr;
-  if (int rc = kv_workspace(ctx, b_max + b_acc + b_done + b_valid + b_sum + (a.score ? 0 : b_keys) + (a.exp_out ? 0 : b_keys), &w)) return rc;
+  if (int rc = kv_workspace(ctx, b_max + b_before + b_acc + b_done + b_valid + b_digits + b_rows + b_weight + b_sum + (a.score ? 0 : b_keys) + (a.exp_out ? 0 : b_keys), &w))
+    return rc;
   char* p = reinterpret_cast<char*>(w);
-  a.chunk_max = reinterpret_cast<int32_t*>(p);
-  p += b_max;
-  a.acc = reinterpret_cast<int64_t*>(p);
-  p += b_acc;
-  a.done = reinterpret_cast<uint32_t*>(p);
-  p += b_done;
-  a.valid = reinterpret_cast<unsigned char*>(p);
-  p += b_valid;
-  if (!a.sum) { a.sum = reinterpret_cast<int64_t*>(p); p += b_sum; }
-  if (!a.score) { a.score = reinterpret_cast<int32_t*>(p); p += b_keys; }
-  if (!a.exp_out) { a.exp_out = reinterpret_cast<int32_t*>(p); p += b_keys; }
-
-  const uint64_t grid = kv_rows * a.tiles * chunks;
-  if (int rc = cache->bits == 32 ? launch_scores<4>(ctx, a, ht, grid, threads, smem) : launch_scores<2>(ctx, a, ht, grid, threads, smem)) return rc;
-  if (int rc = launch(ctx, k_kv_exp, a, rows * exp_chunks, EX_THREADS, 0)) return rc;
-  if (int rc = cache->bits == 32 ? launch_values<4>(ctx, a, v_ht, dones * v_chunks) : launch_values<2>(ctx, a, v_ht, dones * v_chunks)) return rc;
+  auto take = [&](uint64_t bytes) {
+    char* at = p;
+    p += bytes;
+    return reinterpret_cast<void*>(at);
+  };
+  a.piece_max = (int32_t*)take(b_max);
+  a.before = (uint32_t*)take(b_before);
+  a.acc = (int64_t*)take(b_acc);
+  a.done = (uint32_t*)take(b_done);
+  a.valid = (unsigned char*)take(b_valid);
+  a.digits = (unsigned char*)take(b_digits);
+  a.row_at = (int64_t*)take(b_rows);
+  a.weight = (int64_t*)take(b_weight);
+  if (!a.sum) a.sum = (int64_t*)take(b_sum);
+  if (!a.score) a.score = (int32_t*)take(b_keys);
+  if (!a.exp_out) a.exp_out = (int32_t*)take(b_keys);
+  if (int rc = cache->bits == 32 ? launch_scores<4>(ctx, a, threads, smem) : launch_scores<2>(ctx, a, threads, smem)) return rc;
+  if (int rc = launch_softmax(ctx, a, rows, cols)) return rc;
+  if (int rc = cache->bits == 32 ? launch_values<4>(ctx, a, v_grid) : launch_values<2>(ctx, a, v_grid)) return rc;
   GRAPE_CUDA_TRY(ctx, cudaGetLastError());
   return GRAPE_OK;
 }
@@ -784,7 +972,23 @@ extern "C" int grape_kv_attend(grape_ctx* ctx, const grape_kv_cache* cache, cons
   a.softmax = w.d_softmax;
   a.sum = w.d_sum;
   a.out_rem = w.d_out_rem;
-  return attend_launch(ctx, cache, a);
+  // launches of AT_BATCH sequences, one after another on the same workspace
+  for (uint32_t b = 0; b < batch; b += AT_BATCH) {
+    AttendArgs s = a;
+    s.c.batch = std::min(AT_BATCH, batch - b);
+    s.c.table += (uint64_t)b * table_width;
+    s.len += b;
+    s.q += (uint64_t)b * q_stride;
+    if (s.selected) s.selected += (uint64_t)b * cache->kv_heads * n_select;
+    const uint64_t keys = (uint64_t)b * heads * max_keys, channels = (uint64_t)b * heads * cache->head_dim;
+    for (int32_t** p : {&s.score, &s.score_rem, &s.exp_in, &s.exp_out, &s.softmax})
+      if (*p) *p += keys;
+    s.out += channels;
+    if (s.out_rem) s.out_rem += channels;
+    if (s.sum) s.sum += (uint64_t)b * heads;
+    if (int rc = attend_launch(ctx, cache, s)) return rc;
+  }
+  return GRAPE_OK;
 } catch (const std::exception& e) {
   return kv_refuse(nullptr, GRAPE_ERR_NOMEM, "%s", e.what());
 }
