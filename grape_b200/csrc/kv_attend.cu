@@ -72,16 +72,21 @@ __device__ __forceinline__ int32_t column_page(const AttendArgs& a, uint32_t b, 
 // ---- how scores and values are split --------------------------------------------------------------
 // The rows (sequence, key head, head tile, ...) are laid end to end, each cut into sets of 16 or 32 keys, and
 // every block of the grid takes one span of sets, the same number for all: however ragged the lengths, the
-// blocks end together.  A block walks the pieces of the rows that its span covers.  Pieces of row r in block i
-// are numbered r + i: unique, and the pieces of a row lie together.
+// blocks end together.  A row counts for AT_EXTRA sets more than it has, behind its own, which is about what
+// beginning and ending it costs: without them the blocks that meet many short rows end last (32 caches of 301
+// to 4096 tokens: scores 80 us against 65 us for 32 equal ones).  A block walks the pieces of the rows that its
+// span covers.  Pieces of row r in block i are numbered r + i: unique, and the pieces of a row lie together.
 constexpr uint32_t AT_BATCH = 256;  // sequences of a launch
+constexpr uint32_t AT_EXTRA = 8;
 constexpr uint32_t AT_SMEM = 110 * 1024;     // dynamic shared memory of a block that shares its SM with another
 constexpr uint32_t AT_SMEM_ALONE = 222 * 1024;
 
-// s_before[b] = sets of the rows of the sequences before b; returns all of them.
+// s_before[b] = what the rows of the sequences before b count for; returns that of all.
 __device__ __forceinline__ uint32_t plan_sets(const AttendArgs& a, uint32_t* s_before, uint32_t keys, uint32_t rows, bool report) {
-  for (uint32_t b = threadIdx.x; b < a.c.batch; b += blockDim.x)
-    s_before[b + 1] = (columns(a, length(a, b, report)) + keys - 1) / keys * rows;
+  for (uint32_t b = threadIdx.x; b < a.c.batch; b += blockDim.x) {
+    const uint32_t sets = (columns(a, length(a, b, report)) + keys - 1) / keys;
+    s_before[b + 1] = sets ? (sets + AT_EXTRA) * rows : 0;
+  }
   if (threadIdx.x == 0) s_before[0] = 0;
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -102,9 +107,9 @@ __device__ __forceinline__ uint32_t plan_sets(const AttendArgs& a, uint32_t* s_b
 }
 
 struct Piece {
-  uint32_t b, row, sets;         // sequence, row within it, key sets of the whole row
-  uint32_t first_set, count;     // the piece
-  uint32_t begin;                // of the row among all sets
+  uint32_t b, row, sets;      // sequence, row within it, key sets of the whole row
+  uint32_t first_set, count;  // the piece; count may be 0
+  uint32_t begin, next;       // where the row begins, and where the block's span goes on
 };
 __device__ __forceinline__ Piece piece_at(const AttendArgs& a, const uint32_t* s_before, uint32_t rows, uint32_t at, uint32_t end) {
   uint32_t lo = 0, hi = a.c.batch;  // the last b with s_before[b] <= at
@@ -114,13 +119,22 @@ __device__ __forceinline__ Piece piece_at(const AttendArgs& a, const uint32_t* s
   }
   Piece p;
   p.b = lo;
-  p.sets = (s_before[lo + 1] - s_before[lo]) / rows;
-  p.row = (at - s_before[lo]) / p.sets;
-  p.begin = s_before[lo] + p.row * p.sets;
+  const uint32_t units = (s_before[lo + 1] - s_before[lo]) / rows;
+  p.sets = units - AT_EXTRA;
+  p.row = (at - s_before[lo]) / units;
+  p.begin = s_before[lo] + p.row * units;
   p.first_set = at - p.begin;
-  p.count = min(p.sets - p.first_set, end - at);
+  p.next = min(p.begin + units, end);
+  p.count = p.first_set < p.sets ? min(p.sets - p.first_set, end - at) : 0;
   return p;
 }
+
+// ---- one pass after another -----------------------------------------------------------------------------
+// The three passes are launched so that the blocks of the next begin as SMs come free of the last: what they do
+// before after_previous() touches nothing that the pass before writes.  A pass lets the next one begin once
+// its own wait is over, so that whoever runs has all passes before the last one complete behind it.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---- copies ------------------------------------------------------------------------------------------
 // A lane's own queue in shared memory: asynchronous copies that this lane alone reads back, so that no barrier
@@ -223,7 +237,7 @@ __global__ void __launch_bounds__(MT == 2 ? 256 : 512) k_kv_scores(AttendArgs a)
   const char* key[2 * MT];
   auto settle = [&]() {  // on to the piece that holds the warp's next set
     while (ahead_at < end && ahead_k >= ahead.count) {
-      ahead_at += ahead.count;
+      ahead_at = ahead.next;
       ahead_k = team;
       if (ahead_at < end) ahead = piece_at(a, s_before, rows, ahead_at, end);
     }
@@ -289,6 +303,8 @@ __global__ void __launch_bounds__(MT == 2 ? 256 : 512) k_kv_scores(AttendArgs a)
   bool range = false;
   for (uint32_t at = begin; at < end;) {
     const Piece p = piece_at(a, s_before, rows, at, end);
+    at = p.next;
+    if (p.count == 0) continue;
     const uint32_t g = p.row / a.tiles, tile = p.row % a.tiles;
     const uint32_t h0 = g * a.group + tile * HT, hn = min((uint32_t)HT, a.group - tile * HT);
     const uint64_t row0 = (uint64_t)p.b * a.heads + h0;
@@ -413,8 +429,8 @@ __global__ void __launch_bounds__(MT == 2 ? 256 : 512) k_kv_scores(AttendArgs a)
     }
     __syncthreads();
     if (tid < HT) a.piece_max[((uint64_t)p.b * rows + p.row + blockIdx.x) * HT + tid] = s_max[tid];
-    at += p.count;
   }
+  let_next_begin();
   copy_wait<0>();
   if (range) kv_flag(c, STATUS_KV_RANGE);
 }
@@ -438,6 +454,8 @@ __global__ void __launch_bounds__(EX_MAX_THREADS, 2) k_kv_softmax(AttendArgs a, 
   const uint32_t rank = blockIdx.x % blocks, row = blockIdx.x / blocks, h = row % a.heads, b = row / a.heads, g = h / a.group;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, turn = blocks * blockDim.x * EX_COLS;
   const uint32_t cols = columns(a, length(a, b, false));
+  after_previous();
+  let_next_begin();
   if (cols == 0) return;
   const uint32_t first = (rank * warps + warp) * 128 + lane * (ALIGNED ? 4 : 1), up = (cols + 31) & ~31u;
   const uint64_t at = (uint64_t)row * a.max_keys;
@@ -476,8 +494,8 @@ __global__ void __launch_bounds__(EX_MAX_THREADS, 2) k_kv_softmax(AttendArgs a, 
 
   // the row's largest score: its pieces are those of the blocks whose spans it meets
   const uint32_t rows = c.kv_heads * a.tiles, tile = h % a.group / a.score_heads, r = g * a.tiles + tile;
-  const uint32_t before = a.before[b], sets = (a.before[b + 1] - before) / rows, begin = before + r * sets;
-  const uint32_t span = (a.before[c.batch] + a.score_grid - 1) / a.score_grid, first_block = begin / span, last_block = (begin + sets - 1) / span;
+  const uint32_t before = a.before[b], units = (a.before[b + 1] - before) / rows, begin = before + r * units;
+  const uint32_t span = (a.before[c.batch] + a.score_grid - 1) / a.score_grid, first_block = begin / span, last_block = (begin + units - AT_EXTRA - 1) / span;
   int32_t best = INT32_MIN;
   for (uint32_t i = first_block + lane; i <= last_block; i += 32)
     best = max(best, a.piece_max[((uint64_t)b * rows + r + i) * a.score_heads + h % a.group % a.score_heads]);
@@ -485,8 +503,10 @@ __global__ void __launch_bounds__(EX_MAX_THREADS, 2) k_kv_softmax(AttendArgs a, 
 
   int64_t sum = 0;
   bool outside = false;
+  const uint32_t in0 = which(first);
+  int32_t e0[4] = {};  // of the first turn
   for (uint32_t i = first; i < cols; i += turn) {
-    const uint32_t in = which(i);
+    const uint32_t in = i == first ? in0 : which(i);
     int32_t s[4], e[4];
     load(a.score, i, s);
 #pragma unroll
@@ -502,6 +522,7 @@ __global__ void __launch_bounds__(EX_MAX_THREADS, 2) k_kv_softmax(AttendArgs a, 
       if (!(in >> j & 1)) e[j] = 0;
       if (e[j] < 0) { e[j] = 0; outside = true; }
       sum += e[j];
+      if (i == first) e0[j] = e[j];
     }
     store(a.exp_out, i, in, e);
   }
@@ -538,9 +559,14 @@ __global__ void __launch_bounds__(EX_MAX_THREADS, 2) k_kv_softmax(AttendArgs a, 
   unsigned char* const digits = a.digits + (uint64_t)row * 3 * a.padded;
   int64_t weights = 0;
   for (uint32_t i = first; i < up; i += turn) {
-    const uint32_t in = which(i);
+    const uint32_t in = i == first ? in0 : which(i);
     int32_t o[4];
-    load(a.exp_out, i, o);  // this thread's own
+    if (i == first) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] = e0[j];
+    } else {
+      load(a.exp_out, i, o);  // this thread's own
+    }
     uint32_t weight = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -636,7 +662,7 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
       const Piece p = piece_at(a, s_before, rows, ahead_at, end);
       uint32_t g, h0, segment;
       const uint32_t hn = place_of(p.row, g, h0, segment);
-      ahead_at += p.count;
+      ahead_at = p.next;
       if (!hn || p.count <= team) continue;
       ahead_left = (p.count - team + teams - 1) / teams;
       ahead_in = segment * 128 + gl * 16 < row_bytes;
@@ -649,7 +675,13 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
     }
   };
   settle();
-  auto fetch = [&]() {
+  auto fetch_digits = [&](char* to, const unsigned char* from, bool has) {
+    if (has) {
+      copy_async_8(to + my_digits, from);
+      if (NT == 2 && col_digit == 0) copy_async_8(to + my_digits + 256, from + 2 * a.padded);
+    }
+  };
+  auto fetch = [&](bool with_digits) {
     if (ahead_left) {
       char* const to = queue + ahead_stage * VA_STEP;
       const char* from = ahead_base + next_row;
@@ -668,20 +700,29 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
           if (ahead_in) copy_async(to + my_rows + j * 512, ahead_base + row);
         }
       }
-      if (ahead_has) {
-        copy_async_8(to + my_digits, ahead_digits);
-        if (NT == 2 && col_digit == 0) copy_async_8(to + my_digits + 256, ahead_digits + 2 * a.padded);
-      }
+      if (with_digits) fetch_digits(to, ahead_digits, ahead_has);
       ahead_stage = ahead_stage + 1 == VA_STAGES ? 0 : ahead_stage + 1;
       ahead_rows += teams * 32;
       ahead_digits += teams * 32;
       if (--ahead_left) next_row = *ahead_rows;
       else settle();
     }
-    copy_commit();
   };
-#pragma unroll 1
-  for (int i = 0; i < VA_STAGES - 1; i++) fetch();
+  // the rows of the first steps before the softmax is complete, their digits behind it
+  const unsigned char* first_digits[VA_STAGES - 1];
+  bool first_has[VA_STAGES - 1];
+#pragma unroll
+  for (int i = 0; i < VA_STAGES - 1; i++) {
+    first_digits[i] = ahead_digits;
+    first_has[i] = ahead_left && ahead_has;
+    fetch(false);
+  }
+  after_previous();
+#pragma unroll
+  for (int i = 0; i < VA_STAGES - 1; i++) {
+    fetch_digits(queue + i * VA_STEP, first_digits[i], first_has[i]);
+    copy_commit();
+  }
 
   uint32_t stage = 0;
   bool range = false;
@@ -692,7 +733,7 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
       const Piece p = piece_at(a, s_before, rows, at, end);
       uint32_t g, h0, segment;
       count = p.count;
-      at += count;
+      at = p.next;
       if (!place_of(p.row, g, h0, segment) || count <= team) continue;
     }
     int32_t acc[8][NT][4];
@@ -705,7 +746,8 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
       copy_wait<VA_STAGES - 2>();
       const char* const step = queue + stage * VA_STEP;
       stage = stage + 1 == VA_STAGES ? 0 : stage + 1;
-      fetch();  // into the place that was read a step ago
+      fetch(true);  // into the place that was read a step ago
+      copy_commit();
       uint2 d[NT];
 #pragma unroll
       for (int z = 0; z < NT; z++) d[z] = *reinterpret_cast<const uint2*>(step + my_digits + z * 256);
@@ -799,10 +841,28 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
   if (range) kv_flag(c, STATUS_KV_RANGE);
 }
 
-template <class K>
-static int launch(grape_ctx* ctx, K kernel, const AttendArgs& a, uint64_t grid, uint32_t threads, size_t smem) {
+// `overlap`: the blocks may begin before the launch before has ended (see after_previous).
+template <class K, class... Args>
+static int launch(grape_ctx* ctx, K kernel, uint64_t grid, uint32_t threads, size_t smem, uint32_t cluster, bool overlap, const Args&... args) {
   if (smem > 48 * 1024) GRAPE_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<(uint32_t)grid, threads, smem, ctx->stream>>>(a);
+  cudaLaunchAttribute attributes[2] = {};
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((uint32_t)grid);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = ctx->stream;
+  config.attrs = attributes;
+  if (overlap) {
+    attributes[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attributes[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attributes[config.numAttrs].val.clusterDim.x = cluster;
+    attributes[config.numAttrs].val.clusterDim.y = 1;
+    attributes[config.numAttrs++].val.clusterDim.z = 1;
+  }
+  GRAPE_CUDA_TRY(ctx, cudaLaunchKernelEx(&config, kernel, args...));
   ctx->launches += 1;
   return GRAPE_OK;
 }
@@ -812,35 +872,23 @@ static int launch_scores(grape_ctx* ctx, const AttendArgs& a, uint32_t threads, 
   const uint32_t h = a.score_heads;
   auto kernel = a.score_keys == 32 ? (h == 1 ? k_kv_scores<EB, 1, 2> : h == 2 ? k_kv_scores<EB, 2, 2> : k_kv_scores<EB, 4, 2>)
                                    : (h == 1 ? k_kv_scores<EB, 1, 1> : h == 2 ? k_kv_scores<EB, 2, 1> : k_kv_scores<EB, 4, 1>);
-  return launch(ctx, kernel, a, a.score_grid, threads, smem);
+  return launch(ctx, kernel, a.score_grid, threads, smem, 1, false, a);
 }
 
 static int launch_softmax(grape_ctx* ctx, const AttendArgs& a, uint64_t rows, uint64_t cols) {
-  // A thread has its four columns once where the GPU holds that many threads; with more rows than that it takes
-  // turns.  Threads of a block first, up to 1024, then blocks of a cluster, up to 8.
-  const uint64_t room = (uint64_t)ctx->sm_count * 2048 * 2;
+  // As many threads as the GPU holds at a time (phases of several blocks on an SM cover one another), at most one
+  // for every four columns.  Threads of a block first, up to 1024, then blocks of a cluster, up to 8.
+  const uint64_t room = (uint64_t)ctx->sm_count * 2048;
   uint32_t blocks = 1, threads = 256;
   while (threads < EX_MAX_THREADS && (uint64_t)threads * EX_COLS < cols && rows * threads * 2 <= room) threads *= 2;
   while (blocks < 8 && (uint64_t)blocks * threads * EX_COLS < cols && rows * blocks * threads * 2 <= room) blocks *= 2;
-  cudaLaunchAttribute attribute;
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = blocks;
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((uint32_t)(rows * blocks));
-  config.blockDim = dim3(threads);
-  config.stream = ctx->stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  GRAPE_CUDA_TRY(ctx, cudaLaunchKernelEx(&config, a.max_keys % 4 ? k_kv_softmax<false> : k_kv_softmax<true>, a, blocks));
-  ctx->launches += 1;
-  return GRAPE_OK;
+  return launch(ctx, a.max_keys % 4 ? k_kv_softmax<false> : k_kv_softmax<true>, rows * blocks, threads, 0, blocks, true, a, blocks);
 }
 
 template <int EB>
 static int launch_values(grape_ctx* ctx, const AttendArgs& a, uint64_t grid) {
   const uint32_t h = a.v_heads;
-  return launch(ctx, h == 1 ? k_kv_values<EB, 1> : h == 2 ? k_kv_values<EB, 2> : k_kv_values<EB, 4>, a, grid, VA_THREADS, VA_WARPS * VA_STAGES * VA_STEP);
+  return launch(ctx, h == 1 ? k_kv_values<EB, 1> : h == 2 ? k_kv_values<EB, 2> : k_kv_values<EB, 4>, grid, VA_THREADS, VA_WARPS * VA_STAGES * VA_STEP, 1, true, a);
 }
 
 static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs a) {
@@ -863,8 +911,8 @@ static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs
   a.score_heads = ht;
   a.tiles = (a.group + ht - 1) / ht;
   const size_t smem = (size_t)blks * ht * 512 + warps * sc_warp(mt);
-  const uint64_t sets = kv_rows * a.tiles * ((cols + a.score_keys - 1) / a.score_keys);
-  a.score_grid = (uint32_t)std::min<uint64_t>((mt == 2 ? 2 : 1) * sms, sets);
+  const uint64_t units = kv_rows * a.tiles * ((cols + a.score_keys - 1) / a.score_keys + AT_EXTRA);
+  a.score_grid = (uint32_t)std::min<uint64_t>((mt == 2 ? 2 : 1) * sms, units);
 
   // Values: 4 heads a warp, 8 a block where a key head has more than 4 and the segments of a row leave warps for
   // it; up to 8 segments of 128 bytes a block, the rest of a row in other parts; teams share the keys.
@@ -874,12 +922,12 @@ static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs
   a.v_heads = a.group == 1 ? 1 : a.group == 2 ? 2 : a.group <= 4 || a.v_split == VA_WARPS ? 4 : 8;
   a.v_tiles = (a.group + a.v_heads - 1) / a.v_heads;
   a.v_parts = (segments + a.v_split - 1) / a.v_split;
-  const uint64_t v_rows = kv_rows * a.v_parts * a.v_tiles, v_sets = v_rows * ((cols + 31) / 32);
+  const uint64_t v_rows = kv_rows * a.v_parts * a.v_tiles, v_units = v_rows * ((cols + 31) / 32 + AT_EXTRA);
   // a block's span of sets bounds the sums of a register
-  const uint64_t v_grid = std::max<uint64_t>(std::min<uint64_t>(2 * sms, v_sets), (v_sets + VA_SETS - 1) / VA_SETS);
+  const uint64_t v_grid = std::max<uint64_t>(std::min<uint64_t>(2 * sms, v_units), (v_units + VA_SETS - 1) / VA_SETS);
 
   const uint64_t most = 0x7fffffffu;
-  if (sets > most || rows > most || v_sets > most || rows * D > (uint64_t(1) << 38))
+  if (units > most || rows > most || v_units > most || rows * D > (uint64_t(1) << 38))
     return kv_refuse(ctx, GRAPE_ERR_LIMIT, "too many rows and columns for one call");
   a.acc_count = rows * D;
   a.done_count = v_rows * VA_WARPS;
