@@ -121,10 +121,28 @@ struct AppendArgs {
 
 // An item is what one thread handles of a head for every token: 4 channels that lie together or, for the
 // split pairing, two such groups dim/2 apart.
+__host__ __device__ constexpr int ap_stages(bool interleaved) { return interleaved ? 8 : 6; }
+constexpr size_t ap_smem(bool interleaved) { return (size_t)ap_stages(interleaved) * AP_THREADS * (interleaved ? 32 : 64); }
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const int32_t* from) {
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 template <int EB, bool INTERLEAVED>
-__global__ void __launch_bounds__(AP_THREADS) k_kv_append(AppendArgs a) {
+__global__ void __launch_bounds__(AP_THREADS, INTERLEAVED ? 3 : 2) k_kv_append(AppendArgs a) {
   __shared__ int s_b;
-  __shared__ int4 s_red[2][2][AP_THREADS];
+  constexpr int GROUPS = INTERLEAVED ? 1 : 2;  // of four channels that an item has at most
+  extern __shared__ int4 s_queue[];  // [what][stage][thread]
+  auto slot = [&](int what, uint32_t stage) {
+    char* const mine = reinterpret_cast<char*>(s_queue + (what * ap_stages(INTERLEAVED) + stage) * AP_THREADS + threadIdx.x);
+    // with neighbouring pairs a cosine or sine takes 8 bytes: both share the places of one 16-byte tensor
+    return INTERLEAVED && what ? reinterpret_cast<char*>(s_queue + (ap_stages(true) + stage) * AP_THREADS) + (what - 1) * AP_THREADS * 8 + threadIdx.x * 8 : mine;
+  };
   const KvView& c = a.c;
   const uint32_t unit = blockIdx.x, tid = threadIdx.x;
   // units of a sequence begin at offsets[b] / page_size + 2 b: room for every page that its tokens can touch
@@ -179,111 +197,141 @@ __global__ void __launch_bounds__(AP_THREADS) k_kv_append(AppendArgs a) {
   const bool two = !INTERLEAVED && turned;
   const uint32_t shift = kind == 0 ? a.rot_shift + a.k_shift : kind == 1 ? a.v_shift : a.rot_shift;
   const uint32_t up = kind == 1 ? 0 : a.rot_shift;
-  const int32_t* in = kind == 0 ? a.k : kind == 1 ? a.v : a.q;
-  const uint64_t stride = kind == 0 ? a.k_stride : kind == 1 ? a.v_stride : a.q_stride;
-  int32_t* rem = kind == 0 ? a.k_rem : kind == 1 ? a.v_rem : a.q_rem;
   const uint32_t n_heads = kind == 2 ? a.heads : c.kv_heads;
-  char* pool = kind == 0 ? c.k : c.v;
-  const int64_t top = kind == 2 || EB == 4 ? 0x7fffffffll : 0x7fffll;
+  const bool wide = EB == 4 || kind == 2;  // int32 outputs
+  const int64_t top = wide ? 0x7fffffffll : 0x7fffll;
   bool range = false;
-  int32_t low[2][4], high[2][4];
+  int32_t low[GROUPS][4], high[GROUPS][4];
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    low[0][j] = low[1][j] = 0x7fffffff;
-    high[0][j] = high[1][j] = -0x7fffffff - 1;
-  }
-
-  auto finish = [&](const int64_t (&x)[4], int64_t p, uint64_t token, uint32_t at, int which) {
-    int32_t y[4], r[4];
+  for (int w = 0; w < GROUPS; w++)
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const int64_t q = rdiv(x[j], shift);
-      r[j] = (int32_t)(uint32_t)((uint64_t)x[j] - ((uint64_t)q << shift));
-      y[j] = saturate(q, -top - 1, top, range);
-      low[which][j] = min(low[which][j], y[j]);
-      high[which][j] = max(high[which][j], y[j]);
+      low[w][j] = 0x7fffffff;
+      high[w][j] = -0x7fffffff - 1;
     }
-    const uint64_t dense = (token * n_heads + head) * D + at;
-    if (rem) *reinterpret_cast<int4*>(rem + dense) = make_int4(r[0], r[1], r[2], r[3]);
-    if (kind == 2) {
-      *reinterpret_cast<int4*>(a.q_out + dense) = make_int4(y[0], y[1], y[2], y[3]);
-    } else {
-      char* to = pool + page * c.page_stride + head * c.head_stride + (p - page_first) * c.slot_stride + (int64_t)at * EB;
-      if (EB == 4) *reinterpret_cast<int4*>(to) = make_int4(y[0], y[1], y[2], y[3]);
-      else *reinterpret_cast<short4*>(to) = make_short4((short)y[0], (short)y[1], (short)y[2], (short)y[3]);
-    }
-  };
 
   if (active) {
-    constexpr int U = 4;
-    for (int64_t base = p0 + lane; base < p1; base += (int64_t)U * a.lanes) {
-      int4 x[U], x2[U], cs[U], sn[U];
+    // where this thread's first token lies in every tensor, and how far its next one is
+    const uint32_t token0 = (uint32_t)(lo + (p0 - start)) + lane, turns = (uint32_t)(p1 - p0);
+    uint32_t done = lane;
+    const uint64_t in_row = kind == 0 ? a.k_stride : kind == 1 ? a.v_stride : a.q_stride, dense_row = (uint64_t)n_heads * D;
+    const int32_t* in = (kind == 0 ? a.k : kind == 1 ? a.v : a.q) + token0 * in_row + (uint64_t)head * D + ch;
+    int32_t* rem = kind == 0 ? a.k_rem : kind == 1 ? a.v_rem : a.q_rem;
+    const bool with_rem = rem != nullptr;
+    rem += with_rem ? token0 * dense_row + (uint64_t)head * D + ch : 0;
+    char* out = kind == 2 ? reinterpret_cast<char*>(a.q_out + token0 * dense_row + (uint64_t)head * D + ch)
+                          : (kind == 0 ? c.k : c.v) + page * c.page_stride + head * c.head_stride + (p0 + lane - page_first) * c.slot_stride + (int64_t)ch * EB;
+    const uint64_t in_step = in_row * a.lanes, rem_step = dense_row * a.lanes, out_step = (kind == 2 ? dense_row * 4 : (uint64_t)c.slot_stride) * a.lanes;
+    const uint32_t angle = a.rot / 2, angle_step = angle * a.lanes, at0 = INTERLEAVED ? ch / 2 : ch;
+    const int32_t *cos = a.cos + (uint64_t)(p0 + lane) * angle + at0, *sin = a.sin + (uint64_t)(p0 + lane) * angle + at0;
+    const uint32_t apart = a.rot / 2;  // of the two groups of a split pair
+
+    const uint64_t half = (uint64_t(1) << shift) >> 1;
+    const int32_t unit = (int32_t)(0u - (1u << shift));
+    auto finish = [&](const int64_t (&x)[4], int32_t* rem_to, char* to, int which) {
+      int32_t y[4], r[4];
+      uint32_t over = 0;
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int64_t p = base + (int64_t)u * a.lanes;
-        if (p >= p1) continue;
-        const int32_t* row = in + (uint64_t)(lo + (p - start)) * stride + (uint64_t)head * D;
-        x[u] = __ldcs(reinterpret_cast<const int4*>(row + ch));
-        if (two) x2[u] = __ldcs(reinterpret_cast<const int4*>(row + ch2));
+      for (int j = 0; j < 4; j++) {
+        // both words of (x + half) >> shift; it fits 32 bits when the upper one is the lower one's sign
+        const uint64_t sum = (uint64_t)x[j] + half;
+        const uint32_t hi = (uint32_t)(sum >> 32);
+        y[j] = (int32_t)__funnelshift_r((uint32_t)sum, hi, shift);
+        r[j] = y[j] * unit + (int32_t)(uint32_t)(uint64_t)x[j];
+        over |= (uint32_t)((int32_t)hi >> shift) ^ (uint32_t)(y[j] >> 31);
+        if (!wide) over |= (uint32_t)(y[j] ^ (int32_t)(int16_t)y[j]);
+      }
+      if (over) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) y[j] = saturate(rdiv(x[j], shift), -top - 1, top, range);
+      }
+      if (kind == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          low[which][j] = min(low[which][j], y[j]);
+          high[which][j] = max(high[which][j], y[j]);
+        }
+      }
+      if (with_rem) __stcs(reinterpret_cast<int4*>(rem_to), make_int4(r[0], r[1], r[2], r[3]));
+      if (wide) *reinterpret_cast<int4*>(to) = make_int4(y[0], y[1], y[2], y[3]);
+      else *reinterpret_cast<short4*>(to) = make_short4((short)y[0], (short)y[1], (short)y[2], (short)y[3]);
+    };
+    // products of two int32; their sums wrap like unsigned ones
+    auto turn = [](int32_t x0, int32_t x1, int32_t co, int32_t si, int64_t& y0, int64_t& y1) {
+      y0 = (int64_t)((uint64_t)((int64_t)x0 * co) - (uint64_t)((int64_t)x1 * si));
+      y1 = (int64_t)((uint64_t)((int64_t)x1 * co) + (uint64_t)((int64_t)x0 * si));
+    };
+    // The thread's own queue of copies runs AP_STAGES - 1 tokens ahead: what is under way costs no registers.
+    constexpr int STAGES = ap_stages(INTERLEAVED);
+    auto fetch = [&](uint32_t ahead, uint32_t stage) {  // `ahead` in the thread's turns from here
+      if (done + ahead * a.lanes < turns) {
+        const uint64_t n = ahead;
+        copy_async<16>(slot(0, stage), in + n * in_step);
         if (turned) {
-          const uint64_t at = (uint64_t)p * (a.rot / 2) + (INTERLEAVED ? ch / 2 : ch);
-          if (INTERLEAVED) {
-            const int2 cc = __ldg(reinterpret_cast<const int2*>(a.cos + at)), ss = __ldg(reinterpret_cast<const int2*>(a.sin + at));
-            cs[u].x = cc.x; cs[u].y = cc.y; sn[u].x = ss.x; sn[u].y = ss.y;
-          } else {
-            cs[u] = __ldg(reinterpret_cast<const int4*>(a.cos + at));
-            sn[u] = __ldg(reinterpret_cast<const int4*>(a.sin + at));
-          }
+          if (GROUPS == 2) copy_async<16>(slot(1, stage), in + n * in_step + apart);
+          copy_async<INTERLEAVED ? 8 : 16>(slot(GROUPS, stage), cos + n * angle_step);
+          copy_async<INTERLEAVED ? 8 : 16>(slot(GROUPS + 1, stage), sin + n * angle_step);
         }
       }
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int64_t p = base + (int64_t)u * a.lanes;
-        if (p >= p1) continue;
-        const uint64_t token = (uint64_t)(lo + (p - start));
-        const int64_t v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-        int64_t y[4];
-        // products of two int32; their sums wrap like unsigned ones
-        auto turn = [](int64_t x0, int64_t x1, int64_t co, int64_t si, int64_t& y0, int64_t& y1) {
-          y0 = (int64_t)((uint64_t)(x0 * co) - (uint64_t)(x1 * si));
-          y1 = (int64_t)((uint64_t)(x1 * co) + (uint64_t)(x0 * si));
-        };
-        if (!turned) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) y[j] = (int64_t)((uint64_t)v[j] << up);
-          finish(y, p, token, ch, 0);
-        } else if (INTERLEAVED) {
-          turn(v[0], v[1], cs[u].x, sn[u].x, y[0], y[1]);
-          turn(v[2], v[3], cs[u].y, sn[u].y, y[2], y[3]);
-          finish(y, p, token, ch, 0);
-        } else {
-          int64_t z[4];
-          turn(v[0], x2[u].x, cs[u].x, sn[u].x, y[0], z[0]);
-          turn(v[1], x2[u].y, cs[u].y, sn[u].y, y[1], z[1]);
-          turn(v[2], x2[u].z, cs[u].z, sn[u].z, y[2], z[2]);
-          turn(v[3], x2[u].w, cs[u].w, sn[u].w, y[3], z[3]);
-          finish(y, p, token, ch, 0);
-          finish(z, p, token, ch2, 1);
-        }
+      copy_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; i++) fetch(i, i);
+    uint32_t stage = 0;
+#pragma unroll 1
+    for (; done < turns; done += a.lanes) {
+      fetch(STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);  // into the place that was read a turn ago
+      copy_wait<STAGES - 1>();
+      const int4 x = *reinterpret_cast<const int4*>(slot(0, stage));
+      int64_t y[4];
+      if (!turned) {
+        y[0] = (int64_t)((uint64_t)(int64_t)x.x << up);
+        y[1] = (int64_t)((uint64_t)(int64_t)x.y << up);
+        y[2] = (int64_t)((uint64_t)(int64_t)x.z << up);
+        y[3] = (int64_t)((uint64_t)(int64_t)x.w << up);
+        finish(y, rem, out, 0);
+      } else if (INTERLEAVED) {
+        const int2 co = *reinterpret_cast<const int2*>(slot(1, stage)), si = *reinterpret_cast<const int2*>(slot(2, stage));
+        turn(x.x, x.y, co.x, si.x, y[0], y[1]);
+        turn(x.z, x.w, co.y, si.y, y[2], y[3]);
+        finish(y, rem, out, 0);
+      } else {
+        const int4 x2 = *reinterpret_cast<const int4*>(slot(1, stage)), co = *reinterpret_cast<const int4*>(slot(GROUPS, stage)),
+                   si = *reinterpret_cast<const int4*>(slot(GROUPS + 1, stage));
+        int64_t z[4];
+        turn(x.x, x2.x, co.x, si.x, y[0], z[0]);
+        turn(x.y, x2.y, co.y, si.y, y[1], z[1]);
+        turn(x.z, x2.z, co.z, si.z, y[2], z[2]);
+        turn(x.w, x2.w, co.w, si.w, y[3], z[3]);
+        finish(y, rem, out, 0);
+        finish(z, rem + apart, out + apart * (wide ? 4 : EB), GROUPS - 1);
       }
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      in += in_step;
+      rem += rem_step;
+      out += out_step;
+      cos += angle_step;
+      sin += angle_step;
     }
+    copy_wait<0>();
   }
   if (range) kv_flag(c, STATUS_KV_RANGE);
   if (kind != 0 || !c.bounds) return;
 
   // bounds of the page: across the lanes that dealt the tokens out, then into the page's record
+  // (its places of the queue are free: stages 2 w and 2 w + 1 of the first tensor take its group w)
   if (a.lanes > 1) {
 #pragma unroll
-    for (int w = 0; w < 2; w++) {
-      s_red[0][w][tid] = make_int4(low[w][0], low[w][1], low[w][2], low[w][3]);
-      s_red[1][w][tid] = make_int4(high[w][0], high[w][1], high[w][2], high[w][3]);
+    for (int w = 0; w < GROUPS; w++) {
+      *reinterpret_cast<int4*>(slot(0, 2 * w)) = make_int4(low[w][0], low[w][1], low[w][2], low[w][3]);
+      *reinterpret_cast<int4*>(slot(0, 2 * w + 1)) = make_int4(high[w][0], high[w][1], high[w][2], high[w][3]);
     }
     __syncthreads();
     if (lane != 0) return;
     for (uint32_t l = 1; l < a.lanes; l++) {
 #pragma unroll
-      for (int w = 0; w < 2; w++) {
-        const int4 m = s_red[0][w][tid + l * per_block], h = s_red[1][w][tid + l * per_block];
+      for (int w = 0; w < GROUPS; w++) {
+        const int4 m = reinterpret_cast<const int4*>(slot(0, 2 * w))[l * per_block], h = reinterpret_cast<const int4*>(slot(0, 2 * w + 1))[l * per_block];
         low[w][0] = min(low[w][0], m.x); low[w][1] = min(low[w][1], m.y);
         low[w][2] = min(low[w][2], m.z); low[w][3] = min(low[w][3], m.w);
         high[w][0] = max(high[w][0], h.x); high[w][1] = max(high[w][1], h.y);
@@ -293,7 +341,8 @@ __global__ void __launch_bounds__(AP_THREADS) k_kv_append(AppendArgs a) {
   }
   if (!active) return;
   const bool fresh = p0 == page_first;
-  for (int w = 0; w < (two ? 2 : 1); w++) {
+  for (int w = 0; w < GROUPS; w++) {
+    if (w && !two) break;
     char* rec = c.bounds + (((int64_t)page * c.kv_heads + head) * 2 * D + (w ? ch2 : ch)) * EB;
     int32_t l[4], h[4];
 #pragma unroll
@@ -322,9 +371,12 @@ __global__ void __launch_bounds__(AP_THREADS) k_kv_append(AppendArgs a) {
 
 // ---- select ------------------------------------------------------------------------------------
 // bound = max over the group's heads of sum_d max(q_d lo_d, q_d hi_d) = sum_d q_d (q_d >= 0 ? hi_d : lo_d).
-// A group of lanes takes a page's two rows in 16-byte pieces, the queries lie in shared memory.
-constexpr int SB_THREADS = 256;
-constexpr int SB_HEADS = 4;  // heads whose sums a lane holds at a time
+// LANES lanes take the two rows of four pages side by side, in 16-byte pieces: four pages' loads under way (one at a
+// time reached 2.1 TB/s), and four pages x four heads of sums to add up over the lanes, each step of which
+// halves what a lane holds: 32 shuffles for 16 sums where one sum after the other takes 160.
+// What bounds it: bytes of the bounds; a channel and head costs one select and one wide multiply-add.
+constexpr int SB_THREADS = 128;
+constexpr int SB_HEADS = 4, SB_PAGES = 4;  // heads and pages whose sums a lane holds at a time
 
 struct SelectArgs {
   KvView c;
@@ -338,18 +390,21 @@ struct SelectArgs {
   uint32_t chunks, chunk_pages;  // blocks of a row, pages of a block
 };
 
-template <int EB>
-__global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a, uint32_t lanes) {
+template <int EB, int LANES>
+__global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a) {
   extern __shared__ int4 s_q4[];
   const KvView& c = a.c;
   const uint32_t chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, g = row % c.kv_heads, b = row / c.kv_heads;
   const uint32_t D = c.head_dim, vectors = D * EB / 16;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t n = kv_length(c, a.len, b, ~0ull, chunk == 0 && threadIdx.x == 0);
   const uint32_t pages = c.by_page.div(n + c.page_size - 1);
   const uint32_t first = chunk * a.chunk_pages, last = min(pages, first + a.chunk_pages);
   if (first >= last) return;
   const int4* q = reinterpret_cast<const int4*>(a.q + (uint64_t)b * a.q_stride + (uint64_t)g * a.group * D);
-  const uint32_t sub = threadIdx.x & (lanes - 1), per = SB_THREADS / lanes, mine = threadIdx.x / lanes;
+  const uint32_t sub = threadIdx.x % LANES, mine = threadIdx.x / LANES;
+  constexpr uint32_t PER = SB_THREADS / LANES * SB_PAGES;  // pages of the block's turn
+  constexpr int NV = SB_PAGES * SB_HEADS;
   for (uint32_t h0 = 0; h0 < a.group; h0 += SB_HEADS) {
     const uint32_t hn = min((uint32_t)SB_HEADS, a.group - h0);
     __syncthreads();
@@ -357,44 +412,94 @@ __global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a, uint32_t
       s_q4[i] = i < hn * D / 4 ? __ldg(q + (uint64_t)h0 * D / 4 + i) : make_int4(0, 0, 0, 0);
     __syncthreads();
     // whole warps run the loop: the shuffles below need every lane
-    for (uint32_t base = first; base < last; base += per) {
-      const uint32_t i = base + mine;
-      const int32_t page = i < last ? kv_page(c, b, i) : -1;
-      int64_t acc[SB_HEADS] = {};
-      if (page >= 0) {
-        const int4* lo = reinterpret_cast<const int4*>(c.bounds + ((int64_t)page * c.kv_heads + g) * 2 * D * EB);
-        const int4* hi = lo + vectors;
-        for (uint32_t v = sub; v < vectors; v += lanes) {
-          const int4 l4 = __ldg(lo + v), h4 = __ldg(hi + v);
-          const int32_t lw[4] = {l4.x, l4.y, l4.z, l4.w}, hw[4] = {h4.x, h4.y, h4.z, h4.w};
+    for (uint32_t base = first; base < last; base += PER) {
+      const uint32_t i0 = base + mine * SB_PAGES;
+      const int4* rows[SB_PAGES];
+      uint32_t bad = 0;
 #pragma unroll
-          for (int h = 0; h < SB_HEADS; h++) {
-            constexpr int QV = EB == 4 ? 1 : 2;
-            int32_t qq[4 * QV];
+      for (int p = 0; p < SB_PAGES; p++) {
+        int32_t page = i0 + p < last ? kv_page(c, b, i0 + p) : 0;  // a page outside the cache reads page 0 and is dropped
+        if (page < 0) {
+          bad |= 1u << p;
+          page = 0;
+        }
+        rows[p] = reinterpret_cast<const int4*>(c.bounds + ((int64_t)page * c.kv_heads + g) * 2 * D * EB);
+      }
+      uint64_t acc[NV];
 #pragma unroll
-            for (int j = 0; j < QV; j++) {
-              const int4 t = s_q4[h * (D / 4) + v * QV + j];
-              qq[4 * j] = t.x; qq[4 * j + 1] = t.y; qq[4 * j + 2] = t.z; qq[4 * j + 3] = t.w;
-            }
+      for (int k = 0; k < NV; k++) acc[k] = 0;
+#pragma unroll 1
+      for (uint32_t v = sub; v < vectors; v += LANES) {
+        int4 lo[SB_PAGES], hi[SB_PAGES];
 #pragma unroll
-            for (int j = 0; j < 4 * QV; j++) {
-              int32_t x;
-              if (EB == 4) x = qq[j] >= 0 ? hw[j] : lw[j];
-              else x = (int32_t)(int16_t)((uint32_t)(qq[j] >= 0 ? hw[j / 2] : lw[j / 2]) >> (16 * (j & 1)));
-              acc[h] += (int64_t)qq[j] * x;
+        for (int p = 0; p < SB_PAGES; p++) {
+          lo[p] = __ldcs(rows[p] + v);
+          hi[p] = __ldcs(rows[p] + vectors + v);
+        }
+#pragma unroll
+        for (int h = 0; h < SB_HEADS; h++) {
+          constexpr int QV = EB == 4 ? 1 : 2;
+#pragma unroll
+          for (int k = 0; k < QV; k++) {
+            const int4 q4 = s_q4[h * (D / 4) + v * QV + k];
+            const int32_t qq[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const int32_t negative = qq[j] >> 31;  // all ones or none
+#pragma unroll
+              for (int p = 0; p < SB_PAGES; p++) {
+                const int at = EB == 4 ? j : 2 * k + j / 2;
+                const int32_t l = at == 0 ? lo[p].x : at == 1 ? lo[p].y : at == 2 ? lo[p].z : lo[p].w;
+                const int32_t u = at == 0 ? hi[p].x : at == 1 ? hi[p].y : at == 2 ? hi[p].z : hi[p].w;
+                int32_t x = (l & negative) | (u & ~negative);
+                if (EB == 2) x = j & 1 ? x >> 16 : (int32_t)(int16_t)x;
+                acc[p * SB_HEADS + h] += (uint64_t)((int64_t)qq[j] * x);
+              }
             }
           }
         }
       }
+      // the sums over the lanes; a lane keeps the half of its values that its bit of the step names
+      constexpr int STEPS = LANES == 32 ? 5 : LANES == 16 ? 4 : LANES == 8 ? 3 : 2;
+      int held = NV;
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        const int o = LANES >> (s + 1);
+        if (s < 4) {
+          held >>= 1;
+          const bool upper = sub & o;
+#pragma unroll
+          for (int k = 0; k < NV / 2; k++) {
+            if (k >= (NV >> (s + 1))) break;
+            const uint64_t keep = upper ? acc[k + (NV >> (s + 1))] : acc[k], give = upper ? acc[k] : acc[k + (NV >> (s + 1))];
+            acc[k] = keep + __shfl_xor_sync(~0u, give, o);
+          }
+        } else {
+          acc[0] += __shfl_xor_sync(~0u, acc[0], o);
+        }
+      }
+      // values page * SB_HEADS + head: a lane holds NV >> min(STEPS, 4) of them, from this one on
+      constexpr int LEFT = STEPS >= 4 ? 1 : NV >> STEPS;
+      uint32_t at = 0;
+#pragma unroll
+      for (int s = 0; s < (STEPS < 4 ? STEPS : 4); s++)
+        if (sub & (LANES >> (s + 1))) at += NV >> (s + 1);
       int64_t best = INT64_MIN;
 #pragma unroll
-      for (int h = 0; h < SB_HEADS; h++) {
-        for (uint32_t o = lanes / 2; o; o >>= 1) acc[h] += __shfl_xor_sync(~0u, acc[h], o);
-        if (h < (int)hn) best = max(best, acc[h]);
+      for (int k = 0; k < LEFT; k++)
+        if ((at + k) % SB_HEADS < hn) best = max(best, (int64_t)acc[k]);
+      // and the largest over the heads of a page that neighbouring lanes hold
+      if (LEFT == 1) {
+        best = max(best, __shfl_xor_sync(~0u, best, LANES / 16));
+        best = max(best, __shfl_xor_sync(~0u, best, LANES / 8));
+      } else if (LEFT == 2) {
+        best = max(best, __shfl_xor_sync(~0u, best, LANES / 8));
       }
-      if (sub == 0 && i < last) {
+      const uint32_t p = at / SB_HEADS, i = i0 + p;
+      const bool writes = LEFT == 1 ? at % SB_HEADS == 0 && (LANES < 32 || sub % 2 == 0) : at % SB_HEADS == 0;
+      if (writes && i < last) {
         int64_t* to = a.bound + (uint64_t)row * c.width + i;
-        if (page < 0) {
+        if (bad >> p & 1) {
           best = INT64_MIN;
           kv_flag(c, STATUS_KV_PLACE);
         } else if (h0) {
@@ -410,7 +515,7 @@ __global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a, uint32_t
 // below those that are known are counted over the bounds that share them.  Bounds are taken relative to
 // the least, so that the first pass spreads them over its bins.  Then one pass in the pages' order
 // writes what is above that value, the first of what equals it, and the newest pages.
-constexpr int PK_THREADS = 512;
+constexpr int PK_THREADS = 512, PK_HELD = 4;
 
 __device__ __forceinline__ uint32_t block_sum_before(uint32_t flag, uint32_t* s_warp, uint32_t& total) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -440,18 +545,27 @@ __global__ void __launch_bounds__(PK_THREADS) k_kv_pick(SelectArgs a) {
   int32_t* out = a.selected + (uint64_t)row * a.n_select;
   for (uint32_t i = tid; i < a.n_select; i += PK_THREADS)
     if (i >= chosen) out[i] = -1;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the bounds
   if (need >= old) {
     for (uint32_t i = tid; i < chosen; i += PK_THREADS) out[i] = (int32_t)i;
     return;
   }
+  // the first PK_HELD turns' bounds stay in registers
   const int64_t* bound = a.bound + (uint64_t)row * c.width;
-  auto key = [&](uint32_t i) { return (uint64_t)bound[i] ^ (uint64_t(1) << 63); };
+  uint64_t held[PK_HELD];
+#pragma unroll
+  for (int k = 0; k < PK_HELD; k++) held[k] = k * PK_THREADS + tid < old ? (uint64_t)bound[k * PK_THREADS + tid] ^ (uint64_t(1) << 63) : 0;
+  auto for_old = [&](auto&& f) {
+#pragma unroll
+    for (int k = 0; k < PK_HELD; k++)
+      if (k * PK_THREADS + tid < old) f(held[k]);
+    for (uint32_t i = PK_HELD * PK_THREADS + tid; i < old; i += PK_THREADS) f((uint64_t)bound[i] ^ (uint64_t(1) << 63));
+  };
   uint64_t low = ~0ull, high = 0;
-  for (uint32_t i = tid; i < old; i += PK_THREADS) {
-    const uint64_t k = key(i);
+  for_old([&](uint64_t k) {
     low = min(low, k);
     high = max(high, k);
-  }
+  });
   for (int o = 16; o; o >>= 1) {
     low = min(low, __shfl_xor_sync(~0u, low, o));
     high = max(high, __shfl_xor_sync(~0u, high, o));
@@ -472,10 +586,10 @@ __global__ void __launch_bounds__(PK_THREADS) k_kv_pick(SelectArgs a) {
     __syncthreads();
     for (uint32_t i = tid; i < 256; i += PK_THREADS) s_bins[i] = 0;
     __syncthreads();
-    for (uint32_t i = tid; i < old; i += PK_THREADS) {
-      const uint64_t d = key(i) - low;
+    for_old([&](uint64_t k) {
+      const uint64_t d = k - low;
       if (bits == 64 || (d >> bits) == known) atomicAdd(&s_bins[(uint32_t)(d >> shift) & ((1u << w) - 1)], 1u);
-    }
+    });
     __syncthreads();
     if (tid < 32) {
       // lane l holds bins 255-8l .. 248-8l: a scan from the largest digit down
@@ -511,7 +625,7 @@ __global__ void __launch_bounds__(PK_THREADS) k_kv_pick(SelectArgs a) {
     const uint32_t i = base + tid;
     bool above = i >= old && i < pages, tie = false;
     if (i < old) {
-      const uint64_t d = key(i) - low, lead = d >> bits;
+      const uint64_t d = ((uint64_t)bound[i] ^ (uint64_t(1) << 63)) - low, lead = d >> bits;
       above = need != 0 && lead > known;
       tie = need != 0 && lead == known;
     }
@@ -530,23 +644,22 @@ static int append_launch(grape_ctx* ctx, const grape_kv_cache* cache, AppendArgs
   const uint32_t turned = interleaved ? D / 4 : a.rot / 8 + (D - a.rot) / 4;
   a.turned_items = FastDiv::of(turned);
   a.plain_items = FastDiv::of(D / 4);
-  // Lanes that share an item deal a page's tokens out.  One lane each is best when a page receives one
-  // token or the items fill the GPU anyway; few items and many tokens want more.
+  // Lanes that share an item deal a page's tokens out: more, smaller blocks, until there are eight
+  // an SM or a lane would have fewer than eight tokens.
   const uint64_t units = a.tokens / cache->page_size + 2ull * a.c.batch;
   const uint64_t items = (uint64_t)KV * turned + (uint64_t)KV * (D / 4) + (uint64_t)a.heads * turned;
   const uint64_t tokens_per_page = std::min<uint64_t>(cache->page_size, (a.tokens + a.c.batch - 1) / a.c.batch);
   a.lanes = 1;
-  while (a.lanes < 8 && a.lanes * 4 <= tokens_per_page && a.lanes * items * units < (uint64_t)ctx->sm_count * 2048) a.lanes *= 2;
+  while (a.lanes < 4 && a.lanes * 16 <= tokens_per_page && units * items * a.lanes / AP_THREADS < (uint64_t)ctx->sm_count * 4 * 2) a.lanes *= 2;
   const uint64_t per = AP_THREADS / a.lanes;
   a.k_chunks = (uint32_t)(((uint64_t)KV * turned + per - 1) / per);
   a.v_chunks = (uint32_t)(((uint64_t)KV * (D / 4) + per - 1) / per);
   const uint64_t chunks = a.k_chunks + a.v_chunks + (a.q ? ((uint64_t)a.heads * turned + per - 1) / per : 0);
   if (chunks > 65535 || units > 0x7fffffffu) return kv_refuse(ctx, GRAPE_ERR_LIMIT, "too many heads or sequences for one call");
   const dim3 grid((uint32_t)units, (uint32_t)chunks);
-  if (cache->bits == 32 && interleaved) k_kv_append<4, true><<<grid, AP_THREADS, 0, ctx->stream>>>(a);
-  else if (cache->bits == 32) k_kv_append<4, false><<<grid, AP_THREADS, 0, ctx->stream>>>(a);
-  else if (interleaved) k_kv_append<2, true><<<grid, AP_THREADS, 0, ctx->stream>>>(a);
-  else k_kv_append<2, false><<<grid, AP_THREADS, 0, ctx->stream>>>(a);
+  auto kernel = cache->bits == 32 ? (interleaved ? k_kv_append<4, true> : k_kv_append<4, false>) : (interleaved ? k_kv_append<2, true> : k_kv_append<2, false>);
+  GRAPE_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ap_smem(interleaved)));
+  kernel<<<grid, AP_THREADS, ap_smem(interleaved), ctx->stream>>>(a);
   ctx->launches += 1;
   GRAPE_CUDA_TRY(ctx, cudaGetLastError());
   return GRAPE_OK;
@@ -560,16 +673,27 @@ static int select_launch(grape_ctx* ctx, const grape_kv_cache* cache, SelectArgs
     if (int rc = kv_workspace(ctx, rows * a.c.width * sizeof(int64_t), &w)) return rc;
     a.bound = reinterpret_cast<int64_t*>(w);
   }
-  uint32_t lanes = 1;
-  while (lanes < 32 && lanes < D * cache->bits / 8 / 16) lanes *= 2;
+  const uint32_t vectors = D * cache->bits / 8 / 16;
   a.chunk_pages = 64;
   a.chunks = (a.c.width + a.chunk_pages - 1) / a.chunk_pages;
   if (rows * a.chunks > 0x7fffffffu) return kv_refuse(ctx, GRAPE_ERR_LIMIT, "too many pages for one call");
   const size_t smem = (size_t)SB_HEADS * D * 4;
-  auto kernel = cache->bits == 32 ? k_kv_bounds<4> : k_kv_bounds<2>;
+  auto pick = [&](auto k4, auto k2) { return cache->bits == 32 ? k4 : k2; };
+  auto kernel = vectors > 16 ? pick(k_kv_bounds<4, 32>, k_kv_bounds<2, 32>) : vectors > 8 ? pick(k_kv_bounds<4, 16>, k_kv_bounds<2, 16>)
+              : vectors > 4 ? pick(k_kv_bounds<4, 8>, k_kv_bounds<2, 8>) : pick(k_kv_bounds<4, 4>, k_kv_bounds<2, 4>);
   if (smem > 48 * 1024) GRAPE_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<(uint32_t)(rows * a.chunks), SB_THREADS, smem, ctx->stream>>>(a, lanes);
-  k_kv_pick<<<(uint32_t)rows, PK_THREADS, 0, ctx->stream>>>(a);
+  kernel<<<(uint32_t)(rows * a.chunks), SB_THREADS, smem, ctx->stream>>>(a);
+  // the choice may begin while the last bounds are made; it waits for them on the device
+  cudaLaunchAttribute attribute = {};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((uint32_t)rows);
+  config.blockDim = dim3(PK_THREADS);
+  config.stream = ctx->stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  GRAPE_CUDA_TRY(ctx, cudaLaunchKernelEx(&config, k_kv_pick, a));
   ctx->launches += 2;
   GRAPE_CUDA_TRY(ctx, cudaGetLastError());
   return GRAPE_OK;
