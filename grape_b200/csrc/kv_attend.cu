@@ -204,6 +204,41 @@ __device__ __forceinline__ void column_words(const uint64_t (&u)[4 / EB], uint32
 
 constexpr uint32_t SC_SLAB = 1024;  // bytes of a warp's slab of sums
 // A step: 64 bytes of 32 keys (MT = 2), or of 16 where a row is shared by the warps of a block.
+// A block builds the columns of HT heads' queries, hn of them real, in s_w ([blk][HT][32 lanes]: 4 words, those of a
+// lane's 16 bytes), and bias * sum_d q_d of each.  s_bias is zero before.
+template <int EB, int HT>
+__device__ __forceinline__ void build_columns(uint4* s_w, unsigned long long* s_bias, const int32_t* q, uint32_t hn, uint32_t D, uint32_t blks) {
+  constexpr uint32_t PER = 4 / EB;  // elements of a word
+  const uint32_t share = blockDim.x / HT, h = threadIdx.x / share;
+  q += (uint64_t)h * D;
+  int64_t sum = 0;
+  for (uint32_t i = threadIdx.x % share; i < blks * 16; i += share) {
+    uint64_t u[PER];
+#pragma unroll
+    for (uint32_t e = 0; e < PER; e++) {
+      const uint32_t d = i * PER + e;
+      const int32_t v = h < hn && d < D ? __ldg(q + d) : 0;
+      sum += v;
+      u[e] = (uint64_t)((int64_t)v + 0x80808080ll);
+    }
+    // word i of the row: block i / 16, lane group (i / 4) % 4, word i % 4
+    uint32_t* to = reinterpret_cast<uint32_t*>(s_w + ((uint64_t)(i / 16) * HT + h) * 32 + (i / 4) % 4) + i % 4;
+    uint32_t w[8];
+    column_words<EB>(u, w);
+#pragma unroll
+    for (int k = 0; k < 8; k++) to[k * 16] = w[k];
+  }
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  if (threadIdx.x % 32 == 0) atomicAdd(&s_bias[h], (unsigned long long)sum << (EB == 4 ? 31 : 15));
+}
+
+// The eight column sums of a (head, key) at their weights.
+__device__ __forceinline__ uint64_t weigh(const int32_t (&v)[8]) {
+  const int64_t v01 = (int64_t)v[0] + (int64_t)v[1] * 256, v23 = (int64_t)v[2] + (int64_t)v[3] * 256;
+  const int64_t v45 = (int64_t)v[4] + (int64_t)v[5] * 256, v67 = (int64_t)v[6] + (int64_t)v[7] * 256;
+  return (uint64_t)v01 + ((uint64_t)v23 << 16) + ((uint64_t)v45 << 32) + ((uint64_t)v67 << 48);
+}
+
 __host__ __device__ constexpr int sc_stages(int mt) { return mt == 2 ? 5 : 4; }
 __host__ __device__ constexpr uint32_t sc_warp(int mt) { return sc_stages(mt) * mt * 1024 + SC_SLAB; }
 
@@ -311,30 +346,7 @@ __global__ void __launch_bounds__(MT == 2 ? 256 : 512) k_kv_scores(AttendArgs a)
     // the operand columns, and the sum of each head's query
     if (tid < HT) { s_bias[tid] = 0; s_max[tid] = INT32_MIN; }
     __syncthreads();
-    {
-      constexpr uint32_t PER = 4 / EB;  // elements of a word
-      const uint32_t share = blockDim.x / HT, h = tid / share;
-      const int32_t* q = a.q + (uint64_t)p.b * a.q_stride + (uint64_t)(h0 + h) * D;
-      int64_t sum = 0;
-      for (uint32_t i = tid % share; i < blks * 16; i += share) {
-        uint64_t u[PER];
-#pragma unroll
-        for (uint32_t e = 0; e < PER; e++) {
-          const uint32_t d = i * PER + e;
-          const int32_t v = h < hn && d < D ? __ldg(q + d) : 0;
-          sum += v;
-          u[e] = (uint64_t)((int64_t)v + 0x80808080ll);
-        }
-        // word i of the row: block i / 16, lane group (i / 4) % 4, word i % 4
-        uint32_t* to = reinterpret_cast<uint32_t*>(s_dyn + ((uint64_t)(i / 16) * HT + h) * 32 + (i / 4) % 4) + i % 4;
-        uint32_t w[8];
-        column_words<EB>(u, w);
-#pragma unroll
-        for (int k = 0; k < 8; k++) to[k * 16] = w[k];
-      }
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-      if (lane == 0) atomicAdd(&s_bias[h], (unsigned long long)sum << (EB == 4 ? 31 : 15));
-    }
+    build_columns<EB, HT>(s_dyn, s_bias, a.q + (uint64_t)p.b * a.q_stride + (uint64_t)h0 * D, hn, D, blks);
     __syncthreads();
 
     int32_t best[SLABS];
@@ -406,9 +418,7 @@ __global__ void __launch_bounds__(MT == 2 ? 256 : 512) k_kv_scores(AttendArgs a)
           }
           const uint32_t h = MT == 2 ? j : 2 * j + lane / 16;
           if (h < hn && there && (HT * MT >= 2 || lane < 16)) {
-            const int64_t v01 = (int64_t)v[0] + (int64_t)v[1] * 256, v23 = (int64_t)v[2] + (int64_t)v[3] * 256;
-            const int64_t v45 = (int64_t)v[4] + (int64_t)v[5] * 256, v67 = (int64_t)v[6] + (int64_t)v[7] * 256;
-            const uint64_t sum = (uint64_t)v01 + ((uint64_t)v23 << 16) + ((uint64_t)v45 << 32) + ((uint64_t)v67 << 48) - s_bias[h];
+            const uint64_t sum = weigh(v) - s_bias[h];
             const int64_t quotient = rdiv((int64_t)sum, a.score_shift);
             const int32_t score = saturate(quotient, INT32_MIN, INT32_MAX, range);
             const uint64_t to = (row0 + h) * a.max_keys + i;
@@ -503,10 +513,8 @@ __global__ void __launch_bounds__(EX_MAX_THREADS, 2) k_kv_softmax(AttendArgs a, 
 
   int64_t sum = 0;
   bool outside = false;
-  const uint32_t in0 = which(first);
-  int32_t e0[4] = {};  // of the first turn
   for (uint32_t i = first; i < cols; i += turn) {
-    const uint32_t in = i == first ? in0 : which(i);
+    const uint32_t in = which(i);
     int32_t s[4], e[4];
     load(a.score, i, s);
 #pragma unroll
@@ -522,7 +530,6 @@ __global__ void __launch_bounds__(EX_MAX_THREADS, 2) k_kv_softmax(AttendArgs a, 
       if (!(in >> j & 1)) e[j] = 0;
       if (e[j] < 0) { e[j] = 0; outside = true; }
       sum += e[j];
-      if (i == first) e0[j] = e[j];
     }
     store(a.exp_out, i, in, e);
   }
@@ -559,14 +566,9 @@ __global__ void __launch_bounds__(EX_MAX_THREADS, 2) k_kv_softmax(AttendArgs a, 
   unsigned char* const digits = a.digits + (uint64_t)row * 3 * a.padded;
   int64_t weights = 0;
   for (uint32_t i = first; i < up; i += turn) {
-    const uint32_t in = i == first ? in0 : which(i);
+    const uint32_t in = which(i);
     int32_t o[4];
-    if (i == first) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) o[j] = e0[j];
-    } else {
-      load(a.exp_out, i, o);  // this thread's own
-    }
+    load(a.exp_out, i, o);  // this thread's own
     uint32_t weight = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -616,6 +618,63 @@ __device__ __forceinline__ void turn4(uint32_t a, uint32_t b, uint32_t c, uint32
   o[1] = __byte_perm(ab0, cd0, 0x7632);
   o[2] = __byte_perm(ab1, cd1, 0x5410);
   o[3] = __byte_perm(ab1, cd1, 0x7632);
+}
+
+// What a warp of the values' pass holds in its 8 x NT products, channel by channel: f(e, sum) for the 16 / EB channels of
+// the lane's 16 bytes, of head t (NH = 4) or t / 2, every second lane then.  Columns 2t and 2t + 1 of each eight: with
+// four heads digits 0 and 1 of head t lie there and digit 2 in the second eight; with one or two, digit 2 lies in
+// the next lane.
+template <int EB, int NH, int NT, class F>
+__device__ __forceinline__ void each_channel(const int32_t (&acc)[8][NT][4], F&& f) {
+  auto join = [&](uint64_t c0, uint64_t c1, uint64_t c2) {
+    if (NH != 4) c2 = __shfl_xor_sync(~0u, c0, 1);
+    return c0 + (c1 << 8) + (c2 << 16);
+  };
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    uint64_t plane[3][2];  // digit columns: bytes 0 and 1, bytes 2 and 3 of the word
+#pragma unroll
+    for (int z = 0; z < 3; z++) {
+      const int k = z == 2 ? NT - 1 : 0, half = z == 1 ? 1 : 0;
+#pragma unroll
+      for (int m = 0; m < 2; m++)
+        plane[z][m] = (uint64_t)(int64_t)acc[2 * w + m][k][half] + ((uint64_t)(int64_t)acc[2 * w + m][k][2 + half] << 8);
+    }
+    if (EB == 4) {
+      f(w, join(plane[0][0] + (plane[0][1] << 16), plane[1][0] + (plane[1][1] << 16), plane[2][0] + (plane[2][1] << 16)));
+    } else {
+#pragma unroll
+      for (int m = 0; m < 2; m++) f(2 * w + m, join(plane[0][m], plane[1][m], plane[2][m]));
+    }
+  }
+}
+
+// 32 keys x 128 bytes of their values, a lane's 16 bytes of rows 8 t .. 8 t + 7 at from + 512 j, against the digits d.
+// 8 bytes of the rows at a time: all 16 together would not leave registers for two blocks an SM.
+template <int EB, int NT>
+__device__ __forceinline__ void multiply_step(int32_t (&acc)[8][NT][4], const char* from, const uint2 (&d)[NT]) {
+#pragma unroll
+  for (int half = 0; half < 2; half++) {
+    uint2 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = *reinterpret_cast<const uint2*>(from + j * 512 + half * 8);
+#pragma unroll
+    for (int z = 0; z < 2; z++) {
+      const int w = 2 * half + z;
+      uint32_t lo[4], hi[4];
+      auto word = [&](int j) { return z == 0 ? v[j].x : v[j].y; };
+      turn4(word(0), word(1), word(2), word(3), lo);
+      turn4(word(4), word(5), word(6), word(7), hi);
+      lo[3] ^= 0x80808080u;
+      hi[3] ^= 0x80808080u;
+      if (EB == 2) { lo[1] ^= 0x80808080u; hi[1] ^= 0x80808080u; }
+#pragma unroll
+      for (int k = 0; k < NT; k++) {
+        mma_u8u8(acc[2 * w][k], lo[0], lo[1], hi[0], hi[1], d[k].x, d[k].y);
+        mma_u8u8(acc[2 * w + 1][k], lo[2], lo[3], hi[2], hi[3], d[k].x, d[k].y);
+      }
+    }
+  }
 }
 
 // NH: heads of a warp, 1, 2 or 4.  A block takes a.v_heads = NH or 8.
@@ -751,29 +810,7 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
       uint2 d[NT];
 #pragma unroll
       for (int z = 0; z < NT; z++) d[z] = *reinterpret_cast<const uint2*>(step + my_digits + z * 256);
-      // 8 bytes of the rows at a time: all 16 together would not leave registers for two blocks an SM
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
-        uint2 v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = *reinterpret_cast<const uint2*>(step + my_rows + j * 512 + half * 8);
-#pragma unroll
-        for (int z = 0; z < 2; z++) {
-          const int w = 2 * half + z;
-          uint32_t lo[4], hi[4];
-          auto word = [&](int j) { return z == 0 ? v[j].x : v[j].y; };
-          turn4(word(0), word(1), word(2), word(3), lo);
-          turn4(word(4), word(5), word(6), word(7), hi);
-          lo[3] ^= 0x80808080u;
-          hi[3] ^= 0x80808080u;
-          if (EB == 2) { lo[1] ^= 0x80808080u; hi[1] ^= 0x80808080u; }
-#pragma unroll
-          for (int k = 0; k < NT; k++) {
-            mma_u8u8(acc[2 * w][k], lo[0], lo[1], hi[0], hi[1], d[k].x, d[k].y);
-            mma_u8u8(acc[2 * w + 1][k], lo[2], lo[3], hi[2], hi[3], d[k].x, d[k].y);
-          }
-        }
-      }
+      multiply_step<EB, NT>(acc, step + my_rows, d);
     }
     const Piece p = piece_at(a, s_before, rows, here, end);
     uint32_t g, h0, segment;
@@ -781,48 +818,21 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
     // how many sums come together in the row's output: of each of its pieces, the teams that have a set of it
     const uint32_t start = min(p.sets, span - p.begin % span), others = p.sets - start;
     const uint32_t adders = min(teams, start) + others / span * min(teams, span) + min(teams, others % span);
-    // Lane (g, t): columns 2t and 2t + 1 of each eight.  With four heads both digits 0 and 1 of head t lie there and
-    // digit 2 in the second eight; with one or two, digit 2 lies in the next lane.
     const uint32_t head = NH == 4 ? t : t / 2, channel = segment * ELEMS + gl * (16 / EB);
     const bool mine = head < hn && (NH == 4 || t % 2 == 0);
-    constexpr uint64_t BIAS = EB == 4 ? uint64_t(1) << 31 : uint64_t(1) << 15;
-    auto join = [&](uint64_t c0, uint64_t c1, uint64_t c2) {
-      if (NH != 4) c2 = __shfl_xor_sync(~0u, c0, 1);
-      return c0 + (c1 << 8) + (c2 << 16);
-    };
     const uint64_t row = (uint64_t)p.b * a.heads + h0 + (mine ? head : 0), to = row * D + channel;
-    const uint64_t below = BIAS * (uint64_t)a.weight[row];
+    const uint64_t below = (uint64_t)a.weight[row] << (EB == 4 ? 31 : 15);  // bias times the sum of the softmax
     auto finish = [&](uint64_t biased, uint64_t where) {
       const int64_t sum = (int64_t)(biased - below), y = rdiv(sum, a.soft_shift);
       a.out[where] = saturate(y, INT32_MIN, INT32_MAX, range);
       if (a.out_rem) a.out_rem[where] = (int32_t)(uint32_t)((uint64_t)sum - ((uint64_t)y << a.soft_shift));
     };
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-      uint64_t plane[3][2];  // digit columns: bytes 0 and 1, bytes 2 and 3 of the word
-#pragma unroll
-      for (int z = 0; z < 3; z++) {
-        const int k = z == 2 ? NT - 1 : 0, half = z == 1 ? 1 : 0;
-#pragma unroll
-        for (int m = 0; m < 2; m++)
-          plane[z][m] = (uint64_t)(int64_t)acc[2 * w + m][k][half] + ((uint64_t)(int64_t)acc[2 * w + m][k][2 + half] << 8);
+    each_channel<EB, NH, NT>(acc, [&](uint32_t e, uint64_t value) {
+      if (mine && channel + e < D) {
+        if (adders == 1) finish(value, to + e);
+        else atomicAdd(reinterpret_cast<unsigned long long*>(a.acc + to + e), (unsigned long long)value);
       }
-      uint64_t value[4 / EB];
-      if (EB == 4) {
-        value[0] = join(plane[0][0] + (plane[0][1] << 16), plane[1][0] + (plane[1][1] << 16), plane[2][0] + (plane[2][1] << 16));
-      } else {
-#pragma unroll
-        for (int m = 0; m < 4 / EB; m++) value[m] = join(plane[0][m % 2], plane[1][m % 2], plane[2][m % 2]);
-      }
-#pragma unroll
-      for (int m = 0; m < 4 / EB; m++) {
-        const uint32_t e = w * (4 / EB) + m;
-        if (mine && channel + e < D) {
-          if (adders == 1) finish(value[m], to + e);
-          else atomicAdd(reinterpret_cast<unsigned long long*>(a.acc + to + e), (unsigned long long)value[m]);
-        }
-      }
-    }
+    });
     if (adders > 1) {
       // the last of the warps that add to these channels brings the sums to the output
       __threadfence();
@@ -838,6 +848,279 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
     }
   }
   copy_wait<0>();
+  if (range) kv_flag(c, STATUS_KV_RANGE);
+}
+
+// ---- short rows ------------------------------------------------------------------------------------------
+// All three passes over the columns of one head tile by one block: where a key head's rows are short, three launches
+// and their beginnings cost more than the bytes.  Scores, softmax and digits stay in shared memory between the
+// passes; the arithmetic is that of the passes above.
+// Measured against the three passes (us): 32 caches of 64 / 256 / 512 keys, 32 heads on 8 of 128: 15 / 29 / 44 against
+// 31 / 47 / 62; 4 caches of 512: 25 against 27; one cache of 256, 4 heads of 64: 14 against 23.  With few rows and
+// long ones a block alone is too slow: 2 caches of 1024 keys of 16 bits, 16 heads on 4: 31 against 25.
+constexpr uint32_t SM_BYTES = 256 * 1024;     // keys of a row at most
+constexpr uint32_t SM_BYTES_FEW = 128 * 1024; // where there are fewer than SM_MANY blocks
+constexpr uint32_t SM_MANY = 32;
+constexpr int SM_THREADS = 256, SM_WARPS = SM_THREADS / 32, SM_STAGES = 4, SM_VALUE_STAGES = 2;
+constexpr uint32_t SM_QUEUE = 8192;  // bytes of a warp's queue: four steps of keys or two of values
+
+struct SmallLayout {  // of the dynamic shared memory, in bytes
+  uint32_t queue, slabs, row_at, score, digits, valid, all;
+};
+__host__ __device__ inline SmallLayout small_layout(uint32_t blks, uint32_t ht, uint32_t padded) {
+  SmallLayout l;
+  l.queue = blks * ht * 512;
+  l.slabs = l.queue + SM_WARPS * SM_QUEUE;
+  l.row_at = l.slabs + SM_WARPS * SC_SLAB;
+  l.score = l.row_at + padded * 8;
+  l.digits = l.score + ht * padded * 4;
+  l.valid = l.digits + (ht == 4 ? 16 : 8) * (padded + 32);
+  l.all = l.valid + padded;
+  return l;
+}
+
+template <int EB, int HT>
+__global__ void __launch_bounds__(SM_THREADS) k_kv_small(AttendArgs a) {
+  constexpr int SLABS = HT, NT = HT == 4 ? 2 : 1;
+  extern __shared__ uint4 s_dyn[];
+  __shared__ unsigned long long s_bias[HT], s_sum[HT], s_inverse[HT], s_weight[HT];
+  __shared__ int32_t s_max[HT];
+  const KvView& c = a.c;
+  const uint32_t D = c.head_dim, row_bytes = D * EB, blks = (row_bytes + 63) / 64, padded = (uint32_t)a.padded;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, t = lane & 3;
+  const uint32_t tile = blockIdx.x % a.tiles, g = blockIdx.x / a.tiles % c.kv_heads, b = blockIdx.x / a.tiles / c.kv_heads;
+  const uint32_t n = length(a, b, tid == 0 && tile == 0 && g == 0), cols = columns(a, n);
+  const uint32_t h0 = g * a.group + tile * HT, hn = min((uint32_t)HT, a.group - tile * HT);
+  const uint64_t row0 = (uint64_t)b * a.heads + h0;
+  if (cols == 0) {
+    for (uint32_t i = tid; i < hn * D; i += SM_THREADS) {
+      a.out[row0 * D + i] = 0;
+      if (a.out_rem) a.out_rem[row0 * D + i] = 0;
+    }
+    if (a.sum && tid < hn) a.sum[row0 + tid] = 0;
+    return;
+  }
+  const SmallLayout at = small_layout(blks, HT, padded);
+  char* const base = reinterpret_cast<char*>(s_dyn);
+  char* const mine = base + at.queue + warp * SM_QUEUE;
+  char* const slab0 = base + at.slabs + warp * SC_SLAB;
+  int64_t* const s_row = reinterpret_cast<int64_t*>(base + at.row_at);
+  int32_t* const s_score = reinterpret_cast<int32_t*>(base + at.score);
+  unsigned char* const s_digits = reinterpret_cast<unsigned char*>(base + at.digits);
+  unsigned char* const s_valid = reinterpret_cast<unsigned char*>(base + at.valid);
+  const uint32_t sets = (cols + 31) / 32, digits_row = padded + 32;
+
+  // where the columns lie (some row where there is none), and the operand columns
+  if (tid < HT) {
+    s_bias[tid] = s_sum[tid] = s_weight[tid] = 0;
+    s_max[tid] = INT32_MIN;
+  }
+  for (uint32_t i = tid; i < sets * 32; i += SM_THREADS) {
+    uint32_t slot = 0;
+    int32_t page = i < cols ? column_page(a, b, g, n, i, slot, tile == 0) : -1;
+    s_valid[i] = page >= 0;
+    if (page < 0) page = slot = 0;
+    s_row[i] = page * c.page_stride + g * c.head_stride + slot * c.slot_stride;
+  }
+  __syncthreads();
+
+  // scores: a warp every eighth set, `fetch` SM_STAGES - 1 steps of 64 bytes ahead
+  {
+    uint4* const queue = reinterpret_cast<uint4*>(mine) + lane;
+    uint32_t ahead_set = warp, ahead_blk = 0, ahead_stage = 0, stage = 0;
+    auto fetch = [&]() {
+      if (ahead_set < sets) {
+        if (ahead_blk * 64 + t * 16 < row_bytes) {
+#pragma unroll
+          for (int m = 0; m < 4; m++) copy_async(queue + (ahead_stage * 4 + m) * 32, c.k + s_row[ahead_set * 32 + m * 8 + gl] + ahead_blk * 64 + t * 16);
+        }
+        ahead_stage = ahead_stage + 1 == SM_STAGES ? 0 : ahead_stage + 1;
+        if (++ahead_blk == blks) {
+          ahead_blk = 0;
+          ahead_set += SM_WARPS;
+        }
+      }
+      copy_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < SM_STAGES - 1; i++) fetch();
+    build_columns<EB, HT>(s_dyn, s_bias, a.q + (uint64_t)b * a.q_stride + (uint64_t)h0 * D, hn, D, blks);
+    __syncthreads();
+    int32_t best[SLABS];
+#pragma unroll
+    for (int j = 0; j < SLABS; j++) best[j] = INT32_MIN;
+    bool range = false;
+    for (uint32_t set = warp; set < sets; set += SM_WARPS) {
+      int32_t acc[HT][2][4];
+#pragma unroll
+      for (int h = 0; h < HT; h++)
+#pragma unroll
+        for (int m = 0; m < 2; m++) acc[h][m][0] = acc[h][m][1] = acc[h][m][2] = acc[h][m][3] = 0;
+#pragma unroll 1
+      for (uint32_t blk = 0; blk < blks; blk++) {
+        constexpr uint32_t FLIP = EB == 4 ? 0x80000000u : 0x80008000u;
+        copy_wait<SM_STAGES - 2>();
+        uint4 y[4];
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+          y[m] = queue[(stage * 4 + m) * 32];
+          y[m].x ^= FLIP;
+          y[m].y ^= FLIP;
+          y[m].z ^= FLIP;
+          y[m].w ^= FLIP;
+        }
+        stage = stage + 1 == SM_STAGES ? 0 : stage + 1;
+        fetch();  // into the place that was read a step ago
+        const uint4* w = s_dyn + (uint64_t)blk * HT * 32 + lane;
+#pragma unroll
+        for (int h = 0; h < HT; h++) {
+          const uint4 z = w[h * 32];
+#pragma unroll
+          for (int m = 0; m < 2; m++) {
+            mma_u8s8(acc[h][m], y[2 * m].x, y[2 * m + 1].x, y[2 * m].y, y[2 * m + 1].y, z.x, z.y);
+            mma_u8s8(acc[h][m], y[2 * m].z, y[2 * m + 1].z, y[2 * m].w, y[2 * m + 1].w, z.z, z.w);
+          }
+        }
+      }
+      const uint32_t i = set * 32 + lane;
+#pragma unroll
+      for (int j = 0; j < SLABS; j++) {
+        int2* slab = reinterpret_cast<int2*>(slab0);
+#pragma unroll
+        for (int z = 0; z < 4; z++) slab[(z * 8 + gl) * 4 + t] = make_int2(acc[j][z / 2][2 * (z % 2)], acc[j][z / 2][2 * (z % 2) + 1]);
+        __syncwarp();
+        const int4 p0 = reinterpret_cast<const int4*>(slab0)[lane * 2], p1 = reinterpret_cast<const int4*>(slab0)[lane * 2 + 1];
+        const int32_t v[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+        if (j < hn && s_valid[i]) {
+          const uint64_t sum = weigh(v) - s_bias[j];
+          const int64_t quotient = rdiv((int64_t)sum, a.score_shift);
+          const int32_t score = saturate(quotient, INT32_MIN, INT32_MAX, range);
+          const uint64_t to = (row0 + j) * a.max_keys + i;
+          s_score[j * padded + i] = score;
+          if (a.score) a.score[to] = score;
+          if (a.score_rem) a.score_rem[to] = (int32_t)(uint32_t)(sum - ((uint64_t)quotient << a.score_shift));
+          best[j] = max(best[j], score);
+        }
+        __syncwarp();
+      }
+    }
+    copy_wait<0>();
+    if (range) kv_flag(c, STATUS_KV_RANGE);
+#pragma unroll
+    for (int j = 0; j < SLABS; j++) {
+      best[j] = __reduce_max_sync(~0u, best[j]);
+      if (lane == 0) atomicMax(&s_max[j], best[j]);
+    }
+  }
+  __syncthreads();
+
+  // the first values, while the softmax is made
+  const uint32_t segments = (row_bytes + 127) / 128, teams = SM_WARPS / a.v_split, team = warp / a.v_split, segment = warp % a.v_split;
+  const uint32_t my_rows = (t * 8 + (gl ^ (2 * t))) * 16, byte = segment * 128 + gl * 16;
+  uint32_t ahead = team, ahead_stage = 0;
+  auto fetch = [&]() {
+    if (ahead < sets) {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (byte < row_bytes) copy_async(mine + ahead_stage * 4096 + my_rows + j * 512, c.v + s_row[ahead * 32 + 8 * t + j] + byte);
+      ahead_stage = ahead_stage + 1 == SM_VALUE_STAGES ? 0 : ahead_stage + 1;
+      ahead += teams;
+    }
+    copy_commit();
+  };
+#pragma unroll 1
+  for (int i = 0; i < SM_VALUE_STAGES; i++) fetch();
+
+  // softmax: a warp a head (two or eight warps where there are fewer heads)
+  {
+    constexpr uint32_t SHARE = SM_WARPS / HT;
+    const uint32_t h = warp / SHARE, first = warp % SHARE * 32 + lane;
+    const uint64_t to = (row0 + h) * a.max_keys;
+    bool outside = false;
+    if (h < hn) {
+      const int32_t top = s_max[h];
+      int64_t sum = 0;
+      for (uint32_t i = first; i < cols; i += SHARE * 32) {
+        if (!s_valid[i]) continue;
+        const int64_t d = (int64_t)s_score[h * padded + i] - top;
+        outside |= d < a.exp_low;
+        const int32_t x = (int32_t)max(d, (int64_t)a.exp_low);
+        int32_t e = __ldg(a.exp + (x - a.exp_low));
+        if (e < 0) { e = 0; outside = true; }
+        sum += e;
+        s_score[h * padded + i] = e;
+        if (a.exp_in) a.exp_in[to + i] = x;
+        if (a.exp_out) a.exp_out[to + i] = e;
+      }
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+      if (lane == 0) atomicAdd(&s_sum[h], (unsigned long long)sum);
+    }
+    __syncthreads();
+    if (tid < HT) {
+      s_inverse[tid] = s_sum[tid] ? ~0ull / s_sum[tid] : 0;
+      if (tid < hn) {
+        if (a.sum) a.sum[row0 + tid] = (int64_t)s_sum[tid];
+        outside |= s_sum[tid] == 0;
+      }
+    }
+    if (outside) kv_flag(c, STATUS_KV_EXP);
+    __syncthreads();
+    const uint64_t total = s_sum[h], inverse = s_inverse[h];
+    uint64_t weights = 0;
+    for (uint32_t i = first; i < sets * 32; i += SHARE * 32) {
+      uint32_t o = 0;
+      if (h < hn && s_valid[i] && total) {
+        const uint64_t up = ((uint64_t)(uint32_t)s_score[h * padded + i] << a.soft_shift) + total / 2, q = __umul64hi(up, inverse);
+        o = (uint32_t)q + (up - q * total >= total ? 1u : 0u);
+        weights += o;
+      }
+      if (a.softmax && h < hn && s_valid[i]) a.softmax[to + i] = (int32_t)o;
+      // a column of the instruction a digit, as the values' pass has them
+      unsigned char* digits = s_digits + (HT == 4 ? 2 * h : 4 * h) * digits_row + i;
+      digits[0] = (unsigned char)o;
+      digits[digits_row] = (unsigned char)(o >> 8);
+      digits[(HT == 4 ? 8 : 2) * digits_row] = (unsigned char)(o >> 16);
+    }
+    for (int o = 16; o; o >>= 1) weights += __shfl_xor_sync(~0u, weights, o);
+    if (lane == 0) atomicAdd(&s_weight[h], (unsigned long long)weights);
+  }
+  // the columns' places are the sums of the output from here on
+  unsigned long long* const s_out = reinterpret_cast<unsigned long long*>(s_dyn);
+  for (uint32_t i = tid; i < HT * D; i += SM_THREADS) s_out[i] = 0;
+  __syncthreads();
+
+  int32_t acc[8][NT][4];
+#pragma unroll
+  for (int k = 0; k < NT; k++)
+#pragma unroll
+    for (int m = 0; m < 8; m++) acc[m][k][0] = acc[m][k][1] = acc[m][k][2] = acc[m][k][3] = 0;
+  uint32_t stage = 0;
+#pragma unroll 1
+  for (uint32_t set = team; set < sets; set += teams) {
+    copy_wait<SM_VALUE_STAGES - 1>();
+    uint2 d[NT];
+#pragma unroll
+    for (int z = 0; z < NT; z++) d[z] = *reinterpret_cast<const uint2*>(s_digits + (z * 8 + gl) * digits_row + set * 32 + 8 * t);
+    const char* from = mine + stage * 4096 + my_rows;
+    stage = stage + 1 == SM_VALUE_STAGES ? 0 : stage + 1;
+    multiply_step<EB, NT>(acc, from, d);
+    fetch();  // into the place that has just been read
+  }
+  copy_wait<0>();
+  {
+    const uint32_t head = HT == 4 ? t : t / 2, channel = segment * (128 / EB) + gl * (16 / EB);
+    const bool own = head < hn && (HT == 4 || t % 2 == 0) && segment < segments;
+    each_channel<EB, HT, NT>(acc, [&](uint32_t e, uint64_t value) {
+      if (own && channel + e < D) atomicAdd(&s_out[head * D + channel + e], (unsigned long long)value);
+    });
+  }
+  __syncthreads();
+  bool range = false;
+  for (uint32_t i = tid; i < hn * D; i += SM_THREADS) {
+    const int64_t sum = (int64_t)(s_out[i] - (s_weight[i / D] << (EB == 4 ? 31 : 15))), y = rdiv(sum, a.soft_shift);
+    a.out[row0 * D + i] = saturate(y, INT32_MIN, INT32_MAX, range);
+    if (a.out_rem) a.out_rem[row0 * D + i] = (int32_t)(uint32_t)((uint64_t)sum - ((uint64_t)y << a.soft_shift));
+  }
   if (range) kv_flag(c, STATUS_KV_RANGE);
 }
 
@@ -891,11 +1174,30 @@ static int launch_values(grape_ctx* ctx, const AttendArgs& a, uint64_t grid) {
   return launch(ctx, h == 1 ? k_kv_values<EB, 1> : h == 2 ? k_kv_values<EB, 2> : k_kv_values<EB, 4>, grid, VA_THREADS, VA_WARPS * VA_STAGES * VA_STEP, 1, true, a);
 }
 
+template <int EB>
+static int launch_small(grape_ctx* ctx, const AttendArgs& a, uint32_t ht, uint64_t grid, size_t smem) {
+  return launch(ctx, ht == 1 ? k_kv_small<EB, 1> : ht == 2 ? k_kv_small<EB, 2> : k_kv_small<EB, 4>, grid, SM_THREADS, smem, 1, false, a);
+}
+
 static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs a) {
   const uint64_t rows = (uint64_t)a.c.batch * a.heads, D = cache->head_dim, kv_rows = (uint64_t)a.c.batch * cache->kv_heads;
   const uint64_t all = a.selected ? (uint64_t)a.n_select * cache->page_size : (uint64_t)a.c.width * cache->page_size;
   const uint64_t cols = std::min(all, a.max_keys);
   const uint32_t row_bytes = (uint32_t)(D * cache->bits / 8), blks = (row_bytes + 63) / 64, sms = (uint32_t)ctx->sm_count;
+
+  // Short rows: one block for all passes of a head tile, while what it keeps fits an SM.
+  {
+    const uint32_t ht = a.group >= 3 ? 4 : a.group;
+    a.padded = (cols + 31) & ~uint64_t(31);
+    a.tiles = (a.group + ht - 1) / ht;
+    a.v_split = 1;
+    while (a.v_split < 8 && a.v_split < (row_bytes + 127) / 128) a.v_split *= 2;
+    if (row_bytes <= 1024 && a.padded * row_bytes <= (kv_rows * a.tiles < SM_MANY ? SM_BYTES_FEW : SM_BYTES) && kv_rows * a.tiles <= 0x7fffffffu) {
+      const SmallLayout l = small_layout(blks, ht, (uint32_t)a.padded);
+      if (l.all <= AT_SMEM_ALONE && ht * D * 8 <= l.queue)
+        return cache->bits == 32 ? launch_small<4>(ctx, a, ht, kv_rows * a.tiles, l.all) : launch_small<2>(ctx, a, ht, kv_rows * a.tiles, l.all);
+    }
+  }
 
   // Scores.  Rows up to 1 KB: two blocks of 8 warps an SM, a warp a set of 32 keys.  Longer ones: one block of 16
   // warps, 16 keys at a time, a row shared by as many warps as have 8 blocks of it (a few rows of a long head are

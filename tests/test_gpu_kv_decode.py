@@ -329,9 +329,12 @@ def plain_attend(k, v, table, lens, q, exp, low, page, score_shift, soft_shift, 
                 continue
             at = np.array([i for i, _ in cols])
             tok = np.array([t for _, t in cols])
-            kk, vv = (x.view[table[b, tok // page], g, tok % page].astype(object) for x in (k, v))
+            kk, vv = (x.view[table[b, tok // page], g, tok % page] for x in (k, v))
+            # Python integers wherever the products could pass 2^62
+            wide = max(abs(int(kk.min())), abs(int(kk.max()))) * int(np.abs(q[b].astype(np.int64)).max()) * D >= 1 << 62
+            kk, vv = kk.astype(object if wide else np.int64), vv.astype(object if wide else np.int64)
             for h in range(g * (H // KV), (g + 1) * (H // KV)):
-                s, r = rdiv(kk.dot(q[b, h].astype(object)), score_shift)
+                s, r = rdiv(kk.dot(q[b, h].astype(kk.dtype)), score_shift)
                 if max(s) >= 1 << 31 or min(s) < -(1 << 31):
                     status |= 8
                 s = np.clip(s, -(1 << 31), (1 << 31) - 1)
@@ -342,7 +345,7 @@ def plain_attend(k, v, table, lens, q, exp, low, page, score_shift, soft_shift, 
                 z = int(e.sum())
                 status |= 32 if z == 0 else 0
                 o = np.floor_divide(e * (1 << soft_shift) + z // 2, z) if z else e * 0
-                y, yr = rdiv(o.astype(object).dot(vv), soft_shift)
+                y, yr = rdiv(o.astype(vv.dtype).dot(vv), soft_shift)
                 for name, a in (("score", s), ("score_rem", r), ("exp_in", x), ("exp_out", e), ("softmax", o)):
                     out[name][b, h, at] = a
                 if max(y) >= 1 << 31 or min(y) < -(1 << 31):
@@ -391,6 +394,22 @@ ATTEND = [
 ]
 
 
+# rows too long for one block: every width of key rows, one to nine heads a key head, many short sequences beside long ones
+ATTEND_LONG = [
+    ([3001, 40, 2048], 8, 2, 128, 16, 32, "token", 0, 3, 16),
+    ([5000], 2, 1, 64, 32, 24, "head", 0, 0, 16),
+    ([4097, 1], 4, 4, 128, 32, 100, "head", 0, 0, 20),
+    ([2500, 2499, 0, 7], 6, 2, 128, 32, 64, "head", 8, 1, 16),
+    ([3000], 9, 1, 128, 16, 64, "head", 0, 0, 16),
+    ([700, 600], 8, 1, 512, 16, 16, "token", 0, 0, 16),
+    ([700, 601], 3, 1, 512, 32, 7, "head", 0, 0, 16),
+    ([33, 500], 2, 1, 1024, 32, 16, "head", 0, 2, 16),
+    ([40000, 3], 1, 1, 8, 32, 256, "head", 0, 0, 20),
+    ([900] + [5, 0, 1, 17] * 20, 2, 2, 256, 32, 16, "head", 0, 0, 16),
+    ([3, 0, 1, 2] * 66, 1, 1, 520, 32, 8, "head", 0, 1, 16),
+]
+
+
 def attend_setup(gctx, case, kind, seed=21):
     lens, H, KV, D, bits, page, layout, gap, more, soft_shift = case
     rng = np.random.default_rng(seed)
@@ -411,7 +430,7 @@ def attend_setup(gctx, case, kind, seed=21):
     return rng, table, k, v, q, shift, cache
 
 
-@pytest.mark.parametrize("case", ATTEND, ids=str)
+@pytest.mark.parametrize("case", ATTEND + ATTEND_LONG, ids=lambda x: str(x)[:60])
 @pytest.mark.parametrize("kind", ["normal", "extreme"])
 def test_attend(gctx, case, kind):
     lens, H, KV, D, bits, page, layout, gap, more, soft_shift = case
@@ -428,13 +447,13 @@ def test_attend(gctx, case, kind):
     assert np.array_equal(alone["out"], want["out"])
 
 
-@pytest.mark.parametrize("case", ATTEND, ids=str)
+@pytest.mark.parametrize("case", ATTEND + ATTEND_LONG, ids=lambda x: str(x)[:60])
 def test_attend_selected_pages(gctx, case):
     """Lists with holes: nothing selected, the partial page in the middle, a page twice, numbers outside the table."""
     lens, H, KV, D, bits, page, layout, gap, more, soft_shift = case
     rng, table, k, v, q, shift, cache = attend_setup(gctx, case, "normal")
     width = table.shape[1]
-    n_select = min(9, width + 2)
+    n_select = min(9 if case in ATTEND else 60, width + 2)
     sel = rng.integers(-1, width + 1, (len(lens), KV, n_select)).astype(np.int32)
     sel[0, 0, 0] = (lens[0] - 1) // page
     n = 1 << 20
