@@ -86,6 +86,10 @@ class DeviceBuffer:
     def at(self, byte_offset: int) -> int:
         return self.ptr + int(byte_offset)
 
+    @property
+    def _as_parameter_(self):
+        return self.ptr or None    # what ctypes passes for the buffer itself
+
 
 class Context:
     """One GPU, one stream, one scratch arena, one seedable random stream."""
@@ -544,9 +548,9 @@ class Lookup:
         return dict(zip(("A", "S", "B", "T", "m"), vals)), decode_field(u[:n.value])
 
     def close(self):
-        if getattr(self, "handle", None):
+        if getattr(self, "handle", None) and self.ctx.handle:    # a context that is gone took its stream along
             self.ctx.lib.grape_lookup_destroy(self.handle)
-            self.handle = None
+        self.handle = None
 
     def __del__(self):
         try:
