@@ -27,6 +27,7 @@ struct grape_ctx {
   // workspace of the decode-step calls: grow-only, the last block is the current one.  Outgrown blocks are
   // kept until the context goes, since a captured graph may still hold their addresses.
   std::vector<std::pair<void*, size_t>> kv_work;
+  std::vector<const void*> kv_allowed;  // decode-step kernels whose shared memory limit has been raised on this GPU
   // pinned staging buffer for the host-buffer entry points
   void* pinned = nullptr;
   size_t pinned_bytes = 0;

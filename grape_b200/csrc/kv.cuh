@@ -70,6 +70,17 @@ KvView kv_view(grape_ctx* ctx, const grape_kv_cache* c, const int32_t* d_table, 
 // `bytes` of the context's decode-step workspace; the same address for every call that fits the block.
 int kv_workspace(grape_ctx* ctx, size_t bytes, void** out);
 
+// Raises a kernel's limit of dynamic shared memory to `most`, once: the call would cost as much as a launch.
+template <class K>
+inline int kv_allow_shared(grape_ctx* ctx, K* kernel, size_t most) {
+  const void* k = reinterpret_cast<const void*>(kernel);
+  for (const void* have : ctx->kv_allowed)
+    if (have == k) return GRAPE_OK;
+  GRAPE_CUDA_TRY(ctx, cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+  ctx->kv_allowed.push_back(k);
+  return GRAPE_OK;
+}
+
 inline bool misaligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
 }  // namespace grape

@@ -658,7 +658,7 @@ static int append_launch(grape_ctx* ctx, const grape_kv_cache* cache, AppendArgs
   if (chunks > 65535 || units > 0x7fffffffu) return kv_refuse(ctx, GRAPE_ERR_LIMIT, "too many heads or sequences for one call");
   const dim3 grid((uint32_t)units, (uint32_t)chunks);
   auto kernel = cache->bits == 32 ? (interleaved ? k_kv_append<4, true> : k_kv_append<4, false>) : (interleaved ? k_kv_append<2, true> : k_kv_append<2, false>);
-  GRAPE_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ap_smem(interleaved)));
+  if (int rc = kv_allow_shared(ctx, kernel, ap_smem(interleaved))) return rc;
   kernel<<<grid, AP_THREADS, ap_smem(interleaved), ctx->stream>>>(a);
   ctx->launches += 1;
   GRAPE_CUDA_TRY(ctx, cudaGetLastError());
@@ -681,7 +681,8 @@ static int select_launch(grape_ctx* ctx, const grape_kv_cache* cache, SelectArgs
   auto pick = [&](auto k4, auto k2) { return cache->bits == 32 ? k4 : k2; };
   auto kernel = vectors > 16 ? pick(k_kv_bounds<4, 32>, k_kv_bounds<2, 32>) : vectors > 8 ? pick(k_kv_bounds<4, 16>, k_kv_bounds<2, 16>)
               : vectors > 4 ? pick(k_kv_bounds<4, 8>, k_kv_bounds<2, 8>) : pick(k_kv_bounds<4, 4>, k_kv_bounds<2, 4>);
-  if (smem > 48 * 1024) GRAPE_CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (smem > 48 * 1024)
+    if (int rc = kv_allow_shared(ctx, kernel, (size_t)SB_HEADS * 4096 * 4)) return rc;
   kernel<<<(uint32_t)(rows * a.chunks), SB_THREADS, smem, ctx->stream>>>(a);
   // the choice may begin while the last bounds are made; it waits for them on the device
   cudaLaunchAttribute attribute = {};

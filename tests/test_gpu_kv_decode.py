@@ -645,6 +645,48 @@ def test_captured_steps_replay_on_new_data():
     ctx.close()
 
 
+def test_captured_long_rows_replay_on_new_queries():
+    """The three passes of long rows, and the choice of pages, captured together; two replays without waiting between."""
+    import grape_b200
+    import torch
+    from grape_b200 import decode
+    ctx = grape_b200.Context(0)
+    case = ([2500, 2499, 0, 7], 6, 2, 128, 32, 64, "head", 8, 1, 16)
+    rng, table, k, v, q, shift, cache = attend_setup(ctx, case, "normal")
+    lens, H, KV, D, page, n, keys = case[0], 6, 2, 128, 64, 1 << 20, 2500
+    exp = exp_table(n, width=16.0)
+    bounds = np.stack([k.view.min(axis=2), k.view.max(axis=2)], axis=2).copy()
+    cache = decode.KVCache(ctx, k.raw.shape[0], page, KV, D, d_k=cache.k, d_v=cache.v, d_bounds=upload(ctx, bounds), strides=k.strides)
+    d = {name: upload(ctx, a) for name, a in (("table", table), ("len", np.array(lens, np.int32)), ("q", q), ("exp", exp),
+                                              ("out", q), ("sel", np.zeros((4, KV, 5), np.int32)), ("sum", np.zeros((4, H), np.int64)))}
+
+    def issue():
+        decode.kv_select(cache, d["table"], table.shape[1], 4, d["len"], d["q"], H, 5, d["sel"])
+        decode.kv_attend(cache, d["table"], table.shape[1], 4, d["len"], d["q"], H, decode.ExpTable(d["exp"], 1 - n, n), d["out"],
+                         score_shift=shift, max_keys=keys, d_sum=d["sum"])
+
+    issue()
+    ctx.sync()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.ExternalStream(ctx.stream)):
+        issue()
+    for seed in range(3):
+        q = np.rint(np.random.default_rng(seed).normal(0, 65536, q.shape)).astype(np.int32)
+        ctx._check(ctx.lib.grape_h2d(ctx.handle, d["q"].ptr, q.ctypes.data, q.nbytes))
+        ctx.sync()
+        with torch.cuda.stream(torch.cuda.ExternalStream(ctx.stream)):
+            g.replay()
+            g.replay()
+        ctx.sync()
+        sel, _ = plain_select(bounds, table, lens, q, KV, page, 5, 1)
+        want, _ = plain_attend(k, v, table, lens, q, exp, 1 - n, page, shift, 16, keys)
+        assert np.array_equal(fetch(ctx, d["sel"], sel), sel)
+        assert np.array_equal(fetch(ctx, d["out"], want["out"]), want["out"]) and np.array_equal(fetch(ctx, d["sum"], want["sum"]), want["sum"])
+    assert ctx.status() == 0
+    del g
+    ctx.close()
+
+
 def test_a_capture_that_would_have_to_allocate_is_refused():
     import grape_b200
     import torch
