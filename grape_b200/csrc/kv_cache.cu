@@ -372,11 +372,11 @@ __global__ void __launch_bounds__(AP_THREADS, INTERLEAVED ? 3 : 2) k_kv_append(A
 // ---- select ------------------------------------------------------------------------------------
 // bound = max over the group's heads of sum_d max(q_d lo_d, q_d hi_d) = sum_d q_d (q_d >= 0 ? hi_d : lo_d).
 // LANES lanes take the two rows of four pages side by side, in 16-byte pieces: four pages' loads under way (one at a
-// time reached 2.1 TB/s), and four pages x four heads of sums to add up over the lanes, each step of which
+// time reached 2.1 TB/s; eight, for one head, cost registers: 48 us where four take 35), and four pages x four heads of sums to add up over the lanes, each step of which
 // halves what a lane holds: 32 shuffles for 16 sums where one sum after the other takes 160.
 // What bounds it: bytes of the bounds; a channel and head costs one select and one wide multiply-add.
 constexpr int SB_THREADS = 128;
-constexpr int SB_HEADS = 4, SB_PAGES = 4;  // heads and pages whose sums a lane holds at a time
+constexpr int SB_PAGES = 4;  // whose sums a lane holds at a time, for up to four heads
 
 struct SelectArgs {
   KvView c;
@@ -390,9 +390,12 @@ struct SelectArgs {
   uint32_t chunks, chunk_pages;  // blocks of a row, pages of a block
 };
 
-template <int EB, int LANES>
+// SPLIT: the block's warps share the channels of the same pages (and LANES is 32).
+template <int EB, int LANES, int HEADS, bool SPLIT>
 __global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a) {
+  constexpr int WARPS = SB_THREADS / 32;
   extern __shared__ int4 s_q4[];
+  __shared__ uint64_t s_part[SPLIT ? WARPS : 1][SB_PAGES * HEADS];
   const KvView& c = a.c;
   const uint32_t chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks, g = row % c.kv_heads, b = row / c.kv_heads;
   const uint32_t D = c.head_dim, vectors = D * EB / 16;
@@ -402,13 +405,13 @@ __global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a) {
   const uint32_t first = chunk * a.chunk_pages, last = min(pages, first + a.chunk_pages);
   if (first >= last) return;
   const int4* q = reinterpret_cast<const int4*>(a.q + (uint64_t)b * a.q_stride + (uint64_t)g * a.group * D);
-  const uint32_t sub = threadIdx.x % LANES, mine = threadIdx.x / LANES;
-  constexpr uint32_t PER = SB_THREADS / LANES * SB_PAGES;  // pages of the block's turn
-  constexpr int NV = SB_PAGES * SB_HEADS;
-  for (uint32_t h0 = 0; h0 < a.group; h0 += SB_HEADS) {
-    const uint32_t hn = min((uint32_t)SB_HEADS, a.group - h0);
+  const uint32_t sub = threadIdx.x % LANES, mine = SPLIT ? 0 : threadIdx.x / LANES;
+  constexpr uint32_t PER = (SPLIT ? 1 : SB_THREADS / LANES) * SB_PAGES;  // pages of the block's turn
+  constexpr int NV = SB_PAGES * HEADS, LOG = NV == 16 ? 4 : NV == 8 ? 3 : 2;
+  for (uint32_t h0 = 0; h0 < a.group; h0 += HEADS) {
+    const uint32_t hn = min((uint32_t)HEADS, a.group - h0);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < SB_HEADS * D / 4; i += SB_THREADS)
+    for (uint32_t i = threadIdx.x; i < HEADS * D / 4; i += SB_THREADS)
       s_q4[i] = i < hn * D / 4 ? __ldg(q + (uint64_t)h0 * D / 4 + i) : make_int4(0, 0, 0, 0);
     __syncthreads();
     // whole warps run the loop: the shuffles below need every lane
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a) {
 #pragma unroll
       for (int k = 0; k < NV; k++) acc[k] = 0;
 #pragma unroll 1
-      for (uint32_t v = sub; v < vectors; v += LANES) {
+      for (uint32_t v = SPLIT ? threadIdx.x : sub; v < vectors; v += SPLIT ? SB_THREADS : LANES) {
         int4 lo[SB_PAGES], hi[SB_PAGES];
 #pragma unroll
         for (int p = 0; p < SB_PAGES; p++) {
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a) {
           hi[p] = __ldcs(rows[p] + vectors + v);
         }
 #pragma unroll
-        for (int h = 0; h < SB_HEADS; h++) {
+        for (int h = 0; h < HEADS; h++) {
           constexpr int QV = EB == 4 ? 1 : 2;
 #pragma unroll
           for (int k = 0; k < QV; k++) {
@@ -453,7 +456,7 @@ __global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a) {
                 const int32_t u = at == 0 ? hi[p].x : at == 1 ? hi[p].y : at == 2 ? hi[p].z : hi[p].w;
                 int32_t x = (l & negative) | (u & ~negative);
                 if (EB == 2) x = j & 1 ? x >> 16 : (int32_t)(int16_t)x;
-                acc[p * SB_HEADS + h] += (uint64_t)((int64_t)qq[j] * x);
+                acc[p * HEADS + h] += (uint64_t)((int64_t)qq[j] * x);
               }
             }
           }
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a) {
 #pragma unroll
       for (int s = 0; s < STEPS; s++) {
         const int o = LANES >> (s + 1);
-        if (s < 4) {
+        if (s < LOG) {
           held >>= 1;
           const bool upper = sub & o;
 #pragma unroll
@@ -478,25 +481,30 @@ __global__ void __launch_bounds__(SB_THREADS) k_kv_bounds(SelectArgs a) {
           acc[0] += __shfl_xor_sync(~0u, acc[0], o);
         }
       }
-      // values page * SB_HEADS + head: a lane holds NV >> min(STEPS, 4) of them, from this one on
-      constexpr int LEFT = STEPS >= 4 ? 1 : NV >> STEPS;
+      // values page * HEADS + head: a lane holds NV >> min(STEPS, LOG) of them, from this one on
+      constexpr int LEFT = STEPS >= LOG ? 1 : NV >> STEPS;
       uint32_t at = 0;
 #pragma unroll
-      for (int s = 0; s < (STEPS < 4 ? STEPS : 4); s++)
+      for (int s = 0; s < (STEPS < LOG ? STEPS : LOG); s++)
         if (sub & (LANES >> (s + 1))) at += NV >> (s + 1);
+      if (SPLIT) {
+        __syncthreads();  // the turn before has been read
+        s_part[threadIdx.x >> 5][at] = acc[0];
+        __syncthreads();
+        acc[0] = 0;
+        for (int w = 0; w < WARPS; w++) acc[0] += s_part[w][at];
+      }
       int64_t best = INT64_MIN;
 #pragma unroll
       for (int k = 0; k < LEFT; k++)
-        if ((at + k) % SB_HEADS < hn) best = max(best, (int64_t)acc[k]);
+        if (HEADS == 1 || (at + k) % HEADS < hn) best = max(best, (int64_t)acc[k]);
       // and the largest over the heads of a page that neighbouring lanes hold
-      if (LEFT == 1) {
-        best = max(best, __shfl_xor_sync(~0u, best, LANES / 16));
-        best = max(best, __shfl_xor_sync(~0u, best, LANES / 8));
-      } else if (LEFT == 2) {
-        best = max(best, __shfl_xor_sync(~0u, best, LANES / 8));
-      }
-      const uint32_t p = at / SB_HEADS, i = i0 + p;
-      const bool writes = LEFT == 1 ? at % SB_HEADS == 0 && (LANES < 32 || sub % 2 == 0) : at % SB_HEADS == 0;
+#pragma unroll
+      for (int k = 0; (1 << k) < HEADS; k++)
+        if (LOG - k <= STEPS) best = max(best, __shfl_xor_sync(~0u, best, LANES >> (LOG - k)));
+      const uint32_t p = at / HEADS, i = i0 + p;
+      // lanes that hold the same value, and with SPLIT the warps: one of them writes
+      const bool writes = at % HEADS == 0 && (STEPS <= LOG || sub % (LANES >> LOG) == 0) && (!SPLIT || threadIdx.x < 32);
       if (writes && i < last) {
         int64_t* to = a.bound + (uint64_t)row * c.width + i;
         if (bad >> p & 1) {
@@ -674,15 +682,34 @@ static int select_launch(grape_ctx* ctx, const grape_kv_cache* cache, SelectArgs
     a.bound = reinterpret_cast<int64_t*>(w);
   }
   const uint32_t vectors = D * cache->bits / 8 / 16;
-  a.chunk_pages = 64;
+  // Lanes of a page: its row's 16-byte pieces, a warp at most; from 128 pieces on the warps of a block share a page (119
+  // pages of 4096 channels: 12.5 us, a warp a page 22.8).  A block takes up to four turns of its pages while that
+  // leaves eight blocks an SM (16 x 2048 pages of 8 x 128 channels: 68 us, one turn 82, and one turn is what
+  // fills the GPU from 476 pages of 8 heads: 15 us, a fixed 64 pages a block 16.6).  One head or two in a group have kernels of
+  // their own: 4 x 2048 pages of 32 heads with 80 channels of 16 bits take 35 us, with three idle heads 57.
+  const bool split = vectors >= SB_THREADS;
+  const uint32_t lanes = vectors > 16 ? 32 : vectors > 8 ? 16 : vectors > 4 ? 8 : 4, heads = a.group == 1 ? 1 : a.group == 2 ? 2 : 4;
+  const uint32_t turn = (split ? 1 : SB_THREADS / lanes) * SB_PAGES;
+  uint32_t turns = 4;
+  while (turns > 1 && rows * ((a.c.width + turn * turns - 1) / (turn * turns)) < (uint64_t)ctx->sm_count * 8) turns /= 2;
+  a.chunk_pages = turn * turns;
   a.chunks = (a.c.width + a.chunk_pages - 1) / a.chunk_pages;
   if (rows * a.chunks > 0x7fffffffu) return kv_refuse(ctx, GRAPE_ERR_LIMIT, "too many pages for one call");
-  const size_t smem = (size_t)SB_HEADS * D * 4;
+  const size_t smem = (size_t)heads * D * 4;
   auto pick = [&](auto k4, auto k2) { return cache->bits == 32 ? k4 : k2; };
-  auto kernel = vectors > 16 ? pick(k_kv_bounds<4, 32>, k_kv_bounds<2, 32>) : vectors > 8 ? pick(k_kv_bounds<4, 16>, k_kv_bounds<2, 16>)
-              : vectors > 4 ? pick(k_kv_bounds<4, 8>, k_kv_bounds<2, 8>) : pick(k_kv_bounds<4, 4>, k_kv_bounds<2, 4>);
+  auto by_heads = [&](auto h) {
+    constexpr int H = decltype(h)::value;
+    return split         ? pick(k_kv_bounds<4, 32, H, true>, k_kv_bounds<2, 32, H, true>)
+           : lanes == 32 ? pick(k_kv_bounds<4, 32, H, false>, k_kv_bounds<2, 32, H, false>)
+           : lanes == 16 ? pick(k_kv_bounds<4, 16, H, false>, k_kv_bounds<2, 16, H, false>)
+           : lanes == 8  ? pick(k_kv_bounds<4, 8, H, false>, k_kv_bounds<2, 8, H, false>)
+                         : pick(k_kv_bounds<4, 4, H, false>, k_kv_bounds<2, 4, H, false>);
+  };
+  auto kernel = heads == 1   ? by_heads(std::integral_constant<int, 1>())
+                : heads == 2 ? by_heads(std::integral_constant<int, 2>())
+                             : by_heads(std::integral_constant<int, 4>());
   if (smem > 48 * 1024)
-    if (int rc = kv_allow_shared(ctx, kernel, (size_t)SB_HEADS * 4096 * 4)) return rc;
+    if (int rc = kv_allow_shared(ctx, kernel, (size_t)heads * 4096 * 4)) return rc;
   kernel<<<(uint32_t)(rows * a.chunks), SB_THREADS, smem, ctx->stream>>>(a);
   // the choice may begin while the last bounds are made; it waits for them on the device
   cudaLaunchAttribute attribute = {};

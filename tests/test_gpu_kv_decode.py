@@ -248,6 +248,14 @@ SELECT = [
     ([640, 600], 5, 1, 4096, 32, 100, 3, 0),
     ([2100, 2047], 9, 1, 24, 32, 1, 300, 300),
     ([1500], 2, 2, 200, 16, 2, 600, 1),
+    # one head a group and several, for rows of every width: a few 16-byte pieces, warps, blocks
+    ([300, 17], 3, 3, 40, 16, 3, 20, 2),
+    ([800, 90], 2, 2, 1024, 16, 16, 9, 1),
+    ([130], 2, 2, 520, 32, 4, 7, 0),
+    ([333, 12], 6, 2, 1032, 16, 8, 12, 1),
+    ([700, 1], 2, 1, 32, 32, 2, 50, 5),
+    ([5000] * 40, 4, 4, 48, 32, 4, 30, 1),
+    ([6000] * 30, 9, 3, 128, 16, 3, 30, 1),
 ]
 
 
