@@ -201,9 +201,6 @@ __device__ __forceinline__ void column_words(const uint64_t (&u)[4 / EB], uint32
   }
 }
 
-
-constexpr uint32_t SC_SLAB = 1024;  // bytes of a warp's slab of sums
-// A step: 64 bytes of 32 keys (MT = 2), or of 16 where a row is shared by the warps of a block.
 // A block builds the columns of HT heads' queries, hn of them real, in s_w ([blk][HT][32 lanes]: 4 words, those of a
 // lane's 16 bytes), and bias * sum_d q_d of each.  s_bias is zero before.
 template <int EB, int HT>
@@ -239,6 +236,8 @@ __device__ __forceinline__ uint64_t weigh(const int32_t (&v)[8]) {
   return (uint64_t)v01 + ((uint64_t)v23 << 16) + ((uint64_t)v45 << 32) + ((uint64_t)v67 << 48);
 }
 
+// A step: 64 bytes of 32 keys (MT = 2), or of 16 where a row is shared by the warps of a block.
+constexpr uint32_t SC_SLAB = 1024;  // bytes of a warp's slab of sums
 __host__ __device__ constexpr int sc_stages(int mt) { return mt == 2 ? 5 : 4; }
 __host__ __device__ constexpr uint32_t sc_warp(int mt) { return sc_stages(mt) * mt * 1024 + SC_SLAB; }
 
@@ -1184,6 +1183,8 @@ static int attend_launch(grape_ctx* ctx, const grape_kv_cache* cache, AttendArgs
   const uint64_t rows = (uint64_t)a.c.batch * a.heads, D = cache->head_dim, kv_rows = (uint64_t)a.c.batch * cache->kv_heads;
   const uint64_t all = a.selected ? (uint64_t)a.n_select * cache->page_size : (uint64_t)a.c.width * cache->page_size;
   const uint64_t cols = std::min(all, a.max_keys);
+  // without arrays of the caller's, whose rows are max_keys apart, the workspace's rows are as long as a row can be
+  if (!a.score && !a.score_rem && !a.exp_in && !a.exp_out && !a.softmax) a.max_keys = std::min((all + 3) & ~uint64_t(3), a.max_keys);
   const uint32_t row_bytes = (uint32_t)(D * cache->bits / 8), blks = (row_bytes + 63) / 64, sms = (uint32_t)ctx->sm_count;
 
   // Short rows: one block for all passes of a head tile, while what it keeps fits an SM.

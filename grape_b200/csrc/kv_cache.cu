@@ -372,8 +372,9 @@ __global__ void __launch_bounds__(AP_THREADS, INTERLEAVED ? 3 : 2) k_kv_append(A
 // ---- select ------------------------------------------------------------------------------------
 // bound = max over the group's heads of sum_d max(q_d lo_d, q_d hi_d) = sum_d q_d (q_d >= 0 ? hi_d : lo_d).
 // LANES lanes take the two rows of four pages side by side, in 16-byte pieces: four pages' loads under way (one at a
-// time reached 2.1 TB/s; eight, for one head, cost registers: 48 us where four take 35), and four pages x four heads of sums to add up over the lanes, each step of which
-// halves what a lane holds: 32 shuffles for 16 sums where one sum after the other takes 160.
+// time reached 2.1 TB/s; eight, for one head, leave room for fewer warps: 48 us where four take 35), and four pages
+// x four heads of sums to add up over the lanes, each step of which halves what a lane holds: 32 shuffles for
+// 16 sums where one sum after the other takes 160.
 // What bounds it: bytes of the bounds; a channel and head costs one select and one wide multiply-add.
 constexpr int SB_THREADS = 128;
 constexpr int SB_PAGES = 4;  // whose sums a lane holds at a time, for up to four heads

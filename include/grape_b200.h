@@ -375,6 +375,7 @@ const char* grape_static_error(void);
  * fit its type is stored as the type's nearest value and sets a status bit (grape_ctx_status).
  * Device data (lengths, page numbers, positions) is checked on the device: what points outside the
  * cache, the table or the rotation is skipped and sets a status bit, nothing is read or written there.
+ * No output may overlap an input or another output.
  *
  * A cache is the caller's memory: d_k and d_v hold n_pages pages of page_size slots for kv_heads heads of
  * head_dim int16 or int32 values (bits 16 or 32); element (page, head, slot, channel) is at

@@ -499,6 +499,24 @@ def test_attend_bad_pages_lengths_and_tables(gctx):
         assert seen == status == decode.STATUS_EXP and all(np.array_equal(got[name], want[name]) for name in want)
 
 
+def test_any_bound_of_columns_without_a_witness(gctx):
+    """The largest max_keys: the call keeps no more than the table's columns."""
+    from grape_b200 import decode
+    case = ([1500, 900], 8, 2, 64, 32, 16, "head", 0, 0, 16)
+    rng, table, k, v, q, shift, cache = attend_setup(gctx, case, "normal")
+    n = 1 << 20
+    exp = exp_table(n, width=16.0)
+    want, status = plain_attend(k, v, table, [1500, 900], q, exp, 1 - n, 16, shift, 16, 1500)
+    gctx.status()
+    dt, dl, dq, de = (upload(gctx, a) for a in (table, np.array([1500, 900], np.int32), q, exp))
+    out, total = gctx.upload(np.zeros(q.shape, np.int32)), gctx.upload(np.zeros(q.shape[:2], np.int64))
+    decode.kv_attend(cache, dt, table.shape[1], 2, dl, dq, 8, decode.ExpTable(de, 1 - n, n), out, score_shift=shift,
+                     max_keys=(1 << 31) - 1, d_sum=total)
+    assert np.array_equal(fetch(gctx, out, want["out"]), want["out"])
+    assert np.array_equal(fetch(gctx, total, want["sum"]), want["sum"])
+    assert gctx.status() == status
+
+
 def test_offsets_beyond_32_bits(gctx):
     """A cache of three far pages: 2 x 13 GB, elements beyond 2^32."""
     from grape_b200 import decode
