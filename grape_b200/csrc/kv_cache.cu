@@ -81,14 +81,18 @@ int kv_workspace(grape_ctx* ctx, size_t bytes, void** out) {
     GRAPE_CUDA_TRY(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
     if (capture != cudaStreamCaptureStatusNone)
       return kv_refuse(ctx, GRAPE_ERR_NOMEM, "the workspace has to grow to %zu bytes: make one such call outside the capture first", bytes);
-    // at least twice the last block, so that what is kept adds up to less than the current one
+    // twice the last block if there is room, so that what is kept adds up to less than the current one
     size_t want = ctx->kv_work.empty() ? size_t(4) << 20 : 2 * ctx->kv_work.back().second;
     if (want < bytes) want = bytes;
     ctx->kv_work.reserve(ctx->kv_work.size() + 1);
     void* p = nullptr;
     if (cudaMalloc(&p, want) != cudaSuccess) {
       cudaGetLastError();
-      return kv_refuse(ctx, GRAPE_ERR_NOMEM, "workspace of %zu bytes", want);
+      want = bytes;  // what the call needs may still be there
+      if (cudaMalloc(&p, want) != cudaSuccess) {
+        cudaGetLastError();
+        return kv_refuse(ctx, GRAPE_ERR_NOMEM, "workspace of %zu bytes", want);
+      }
     }
     ctx->kv_work.push_back({p, want});
   }

@@ -748,6 +748,29 @@ def test_two_contexts_at_once():
     b.close()
 
 
+def test_the_workspace_takes_what_there_is():
+    """Where twice the last workspace finds no room, the call gets what it needs."""
+    import torch
+    from grape_b200 import decode, host
+    ctx = host.Context(0)
+    width = (40 << 20, 50 << 20)                                  # 8 bytes a page of the table: 320 and 400 MB
+    cache = decode.KVCache(ctx, 1, 1, 1, 8)
+    dt, dl = ctx.alloc(width[1] * 4), ctx.upload(np.zeros(1, np.int32))
+    dq, ds = ctx.upload(np.ones(8, np.int32)), ctx.upload(np.zeros(2, np.int32))
+    torch.cuda.empty_cache()
+    hold = torch.empty(torch.cuda.mem_get_info()[0] - (900 << 20), dtype=torch.uint8, device="cuda")
+    for w in width:
+        decode.kv_select(cache, dt, w, 1, dl, dq, 1, 2, ds)
+        assert ctx.download(ds, 8, np.int32).tolist() == [-1, -1]
+    with pytest.raises(host.GrapeError, match="workspace"):
+        decode.kv_select(cache, dt, 1 << 30, 1, dl, dq, 1, 2, ds)
+    assert ctx.status() == 0
+    del hold
+    torch.cuda.empty_cache()
+    cache.close()
+    ctx.close()
+
+
 def test_empty_calls(gctx):
     from grape_b200 import decode
     cache = decode.KVCache(gctx, 1, 16, 1, 64)
