@@ -1126,7 +1126,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_kv_small(AttendArgs a) {
 // `overlap`: the blocks may begin before the launch before has ended (see after_previous).
 template <class K, class... Args>
 static int launch(grape_ctx* ctx, K kernel, uint64_t grid, uint32_t threads, size_t smem, uint32_t cluster, bool overlap, const Args&... args) {
-  if (smem > 48 * 1024)
+  if (smem)  // the limit of 48 KB is for this and the kernel's own arrays together
     if (int rc = kv_allow_shared(ctx, kernel, AT_SMEM_ALONE)) return rc;
   cudaLaunchAttribute attributes[2] = {};
   cudaLaunchConfig_t config = {};

@@ -713,9 +713,11 @@ static int select_launch(grape_ctx* ctx, const grape_kv_cache* cache, SelectArgs
   auto kernel = heads == 1   ? by_heads(std::integral_constant<int, 1>())
                 : heads == 2 ? by_heads(std::integral_constant<int, 2>())
                              : by_heads(std::integral_constant<int, 4>());
-  if (smem > 48 * 1024)
-    if (int rc = kv_allow_shared(ctx, kernel, (size_t)heads * 4096 * 4)) return rc;
+  // The limit of 48 KB is for the queries and the kernel's own sums together: the widest head's need, for every width.
+  if (int rc = kv_allow_shared(ctx, kernel, (size_t)heads * 4096 * 4)) return rc;
   kernel<<<(uint32_t)(rows * a.chunks), SB_THREADS, smem, ctx->stream>>>(a);
+  GRAPE_CUDA_TRY(ctx, cudaGetLastError());  // no choice over bounds that were not made
+  ctx->launches += 1;
   // the choice may begin while the last bounds are made; it waits for them on the device
   cudaLaunchAttribute attribute = {};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -727,7 +729,7 @@ static int select_launch(grape_ctx* ctx, const grape_kv_cache* cache, SelectArgs
   config.attrs = &attribute;
   config.numAttrs = 1;
   GRAPE_CUDA_TRY(ctx, cudaLaunchKernelEx(&config, k_kv_pick, a));
-  ctx->launches += 2;
+  ctx->launches += 1;
   GRAPE_CUDA_TRY(ctx, cudaGetLastError());
   return GRAPE_OK;
 }
