@@ -69,6 +69,9 @@ __device__ __forceinline__ int32_t column_page(const AttendArgs& a, uint32_t b, 
   return page;
 }
 
+// Entry of the exp table for an argument in [exp_low, 0]: up to 2^31, so the difference is an unsigned one.
+__device__ __forceinline__ uint32_t exp_index(const AttendArgs& a, int32_t x) { return (uint32_t)x - (uint32_t)a.exp_low; }
+
 // ---- how scores and values are split --------------------------------------------------------------
 // The rows (sequence, key head, head tile, ...) are laid end to end, each cut into sets of 16 or 32 keys, and
 // every block of the grid takes one span of sets, the same number for all: however ragged the lengths, the
@@ -521,7 +524,7 @@ __global__ void __launch_bounds__(EX_MAX_THREADS, 2) k_kv_softmax(AttendArgs a, 
       const int64_t d = in >> j & 1 ? (int64_t)s[j] - best : 0;
       outside |= d < a.exp_low;
       s[j] = (int32_t)max(d, (int64_t)a.exp_low);
-      e[j] = __ldg(a.exp + (s[j] - a.exp_low));
+      e[j] = __ldg(a.exp + exp_index(a, s[j]));
     }
     store(a.exp_in, i, in, s);
 #pragma unroll
@@ -1044,7 +1047,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_kv_small(AttendArgs a) {
         const int64_t d = (int64_t)s_score[h * padded + i] - top;
         outside |= d < a.exp_low;
         const int32_t x = (int32_t)max(d, (int64_t)a.exp_low);
-        int32_t e = __ldg(a.exp + (x - a.exp_low));
+        int32_t e = __ldg(a.exp + exp_index(a, x));
         if (e < 0) { e = 0; outside = true; }
         sum += e;
         s_score[h * padded + i] = e;
