@@ -149,20 +149,52 @@ __global__ void __launch_bounds__(AP_THREADS, INTERLEAVED ? 3 : 2) k_kv_append(A
   };
   const KvView& c = a.c;
   const uint32_t unit = blockIdx.x, tid = threadIdx.x;
-  // units of a sequence begin at offsets[b] / page_size + 2 b: room for every page that its tokens can touch
+  // Units of a sequence begin at offsets[b] / page_size + 2 b: room for every page that its tokens can touch, and units
+  // of its own as long as offsets do not fall.  A sequence whose rows do not lie in the call's has none.
   if (tid == 0) s_b = -1;
   __syncthreads();
+  bool falls = false, outside = false;
+  auto rows_of = [&](uint32_t b, int64_t& lo, int64_t& hi) {
+    lo = __ldg(a.offsets + b);
+    hi = __ldg(a.offsets + b + 1);
+    falls |= hi < lo;
+    return lo >= 0 && hi >= lo && hi <= a.tokens;
+  };
+  auto has_unit = [&](uint32_t b, int64_t lo, int64_t hi) {
+    const uint64_t first = (uint64_t)c.by_page.div((uint32_t)lo) + 2ull * b, next = (uint64_t)c.by_page.div((uint32_t)hi) + 2ull * b + 2;
+    return unit >= first && unit < next;
+  };
   for (uint32_t b = tid; b < c.batch; b += AP_THREADS) {
-    const uint32_t lo = (uint32_t)__ldg(a.offsets + b), hi = (uint32_t)__ldg(a.offsets + b + 1);
-    const uint64_t first = (uint64_t)c.by_page.div(lo & 0x7fffffffu) + 2ull * b;
-    const uint64_t next = (uint64_t)c.by_page.div(hi & 0x7fffffffu) + 2ull * b + 2;
-    if (unit >= first && unit < next) s_b = (int)b;
+    int64_t lo, hi;
+    const bool in = rows_of(b, lo, hi);
+    outside |= !in;
+    if (in && has_unit(b, lo, hi)) s_b = (int)b;
   }
-  __syncthreads();
+  if (outside && unit == 0 && blockIdx.y == 0) kv_flag(c, STATUS_KV_PLACE);
+  if (__syncthreads_or(falls)) {
+    // of the sequences that claim the same rows the first has them; one warp finds the block's again
+    if (tid == 0) s_b = -1;
+    __syncthreads();
+    int64_t taken = 0;
+    for (uint32_t base = 0; tid < 32 && base < c.batch; base += 32) {
+      int64_t lo = 0, hi = 0;
+      const bool in = base + tid < c.batch && rows_of(base + tid, lo, hi);
+      int64_t upto = in ? hi : 0;  // the largest end so far
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t before = __shfl_up_sync(~0u, upto, o);
+        if ((int)tid >= o) upto = max(upto, before);
+      }
+      int64_t before = __shfl_up_sync(~0u, upto, 1);
+      before = max(taken, tid ? before : 0);
+      if (in && lo >= before && has_unit(base + tid, lo, hi)) s_b = (int)(base + tid);
+      taken = max(taken, __shfl_sync(~0u, upto, 31));
+    }
+    __syncthreads();
+  }
   if (s_b < 0) return;
   const uint32_t b = (uint32_t)s_b;
   const int64_t lo = __ldg(a.offsets + b), hi = __ldg(a.offsets + b + 1), start = __ldg(a.start + b);
-  if (lo < 0 || hi < lo || hi > a.tokens || start < 0) {
+  if (start < 0) {
     if (tid == 0) kv_flag(c, STATUS_KV_PLACE);
     return;
   }

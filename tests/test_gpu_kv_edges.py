@@ -2,9 +2,85 @@
 import numpy as np
 import pytest
 
-from test_gpu_kv_decode import WITNESS, Pool, fetch, make_cache, plain_attend, plain_select, table_for, upload
+from test_gpu_kv_decode import (WITNESS, Pool, fetch, make_cache, plain_append, plain_attend, plain_select, table_for,
+                                upload)
 
 pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------- append
+def taken_sequences(offsets, tokens):
+    """Sequences whose rows lie in the call's and, where offsets fall, behind those of the sequences before."""
+    got, end = [], 0
+    for b, (lo, hi) in enumerate(zip(offsets[:-1], offsets[1:])):
+        if 0 <= lo <= hi <= tokens:
+            if lo >= end:
+                got.append(b)
+            end = max(end, hi)
+    return got
+
+
+def scattered_offsets(n, tokens, seed):
+    """Offsets of n sequences, a few of which fall, lie below 0 or behind the rows."""
+    rng = np.random.default_rng(seed)
+    o = np.sort(rng.integers(0, tokens + 1, n + 1))
+    at = rng.choice(n + 1, 5, replace=False)
+    o[at] = rng.integers(-50, tokens + 50, 5)
+    return [int(x) for x in o]
+
+
+OFFSETS = [
+    # offsets, sequences that are appended
+    ([-1, 10, 24], [1]),
+    ([0, 24, 2, 24], [0]),
+    ([0, 20, 2, 24], [0]),
+    ([0, 10, 5, 24], [0]),
+    ([8, 3, 3, 24], [1, 2]),
+    ([0, 30, 10, 24], [2]),
+    ([40, 50, 24], []),
+    ([0, 8, 8, 16, 4, 24], [0, 1, 2]),
+    ([0, 24, -(1 << 31), 24], [0]),
+    ([0, (1 << 31) - 1, 8, 24], [2]),
+    ([0, 6, 6, 24, 24], [0, 1, 2, 3]),
+    ([5, 9, 20], [0, 1]),
+    (scattered_offsets(40, 300, 1), None),
+    (scattered_offsets(700, 900, 2), None),
+    (scattered_offsets(700, 900, 3), None),
+]
+
+
+@pytest.mark.parametrize("offsets, want_taken", OFFSETS, ids=lambda x: str(x)[:30])
+def test_append_with_bad_offsets(gctx, offsets, want_taken):
+    """A sequence whose rows lie outside or run backwards is skipped and reported, wherever it stands; of sequences that
+    share rows the first has them; all others are appended."""
+    from grape_b200 import decode
+    rng = np.random.default_rng(8)
+    tokens = 24 if want_taken is not None else 300 if len(offsets) == 41 else 900
+    taken = taken_sequences(offsets, tokens)
+    assert want_taken is None or taken == want_taken
+    B, KV, D, page = len(offsets) - 1, 2, 8, 8
+    start = [(4 + 5 * b) % 11 for b in range(B)]
+    ends = [s + max(0, min(hi, tokens) - max(lo, 0)) for s, lo, hi in zip(start, offsets[:-1], offsets[1:])]
+    P = sum(-(-n // page) for n in ends) + 2
+    table = table_for(rng, P, ends, page)
+    k, v = (Pool(rng, P, KV, page, D, 32) for _ in range(2))
+    bounds = np.stack([k.view.min(axis=2), k.view.max(axis=2)], axis=2).copy()
+    x = rng.integers(-1000, 1000, (tokens, 2, KV, D)).astype(np.int32)
+    cache = make_cache(gctx, k, v, page, KV, D, 32, bounds=bounds)
+    dx, dt, ds, do = (upload(gctx, a) for a in (x, table, np.array(start, np.int32), np.array(offsets, np.int32)))
+    rem = gctx.upload(np.full((tokens, KV, D), 5, np.int32))
+    gctx.status()
+    decode.kv_append(cache, dt, table.shape[1], B, ds, do, tokens, dx, dx.at(4 * KV * D), k_stride=2 * KV * D, v_stride=2 * KV * D,
+                     d_k_rem=rem)
+    whole = all(0 <= lo <= hi <= tokens for lo, hi in zip(offsets[:-1], offsets[1:]))
+    assert gctx.status() == (0 if whole else decode.STATUS_PLACE)
+    want = np.full((tokens, KV, D), 5, np.int32)
+    for b in taken:
+        plain_append(k, v, bounds, table[b:b + 1], [start[b]], offsets[b:b + 2], x[:, 0], x[:, 0], x[:, 1], None, None, 0, 0, True, 0, 0, page)
+        want[offsets[b]:offsets[b + 1]] = 0
+    assert np.array_equal(fetch(gctx, rem, want), want)
+    assert np.array_equal(fetch(gctx, cache.k, k.raw), k.raw) and np.array_equal(fetch(gctx, cache.v, v.raw), v.raw)
+    assert np.array_equal(fetch(gctx, cache.bounds, bounds), bounds)
 
 
 # ---------------------------------------------------------------------------------- select
