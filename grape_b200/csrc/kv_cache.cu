@@ -106,6 +106,9 @@ int kv_workspace(grape_ctx* ctx, size_t bytes, void** out) {
 // on the tokens that ONE page receives, so that the page's bounds are a reduction inside the block and
 // one plain read-modify-write: no atomics, and no order that could change them.
 constexpr int AP_THREADS = 256;
+// Sequences of a launch: every block looks through all of them for its own, so a batch of many times as many in one launch
+// would cost their square (one token for each of 4096 and 262144 sequences: 0.12 and 302 ms, in launches of 1024 0.10 and 10).
+constexpr uint32_t AP_BATCH = 1024;
 
 struct AppendArgs {
   KvView c;
@@ -154,18 +157,18 @@ __global__ void __launch_bounds__(AP_THREADS, INTERLEAVED ? 3 : 2) k_kv_append(A
   if (tid == 0) s_b = -1;
   __syncthreads();
   bool falls = false, outside = false;
-  auto rows_of = [&](uint32_t b, int64_t& lo, int64_t& hi) {
+  auto rows_of = [&](uint32_t b, int32_t& lo, int32_t& hi) {
     lo = __ldg(a.offsets + b);
     hi = __ldg(a.offsets + b + 1);
     falls |= hi < lo;
-    return lo >= 0 && hi >= lo && hi <= a.tokens;
+    return lo >= 0 && hi >= lo && (uint32_t)hi <= a.tokens;
   };
-  auto has_unit = [&](uint32_t b, int64_t lo, int64_t hi) {
-    const uint64_t first = (uint64_t)c.by_page.div((uint32_t)lo) + 2ull * b, next = (uint64_t)c.by_page.div((uint32_t)hi) + 2ull * b + 2;
-    return unit >= first && unit < next;
+  auto has_unit = [&](uint32_t b, int32_t lo, int32_t hi) {  // lo / page_size + 2 b <= unit < hi / page_size + 2 b + 2
+    const int64_t row = (int64_t)((int32_t)unit - 2 * (int32_t)b) * (int32_t)c.page_size;
+    return lo < row + c.page_size && hi >= row - c.page_size;
   };
   for (uint32_t b = tid; b < c.batch; b += AP_THREADS) {
-    int64_t lo, hi;
+    int32_t lo, hi;
     const bool in = rows_of(b, lo, hi);
     outside |= !in;
     if (in && has_unit(b, lo, hi)) s_b = (int)b;
@@ -175,16 +178,16 @@ __global__ void __launch_bounds__(AP_THREADS, INTERLEAVED ? 3 : 2) k_kv_append(A
     // of the sequences that claim the same rows the first has them; one warp finds the block's again
     if (tid == 0) s_b = -1;
     __syncthreads();
-    int64_t taken = 0;
+    int32_t taken = 0;
     for (uint32_t base = 0; tid < 32 && base < c.batch; base += 32) {
-      int64_t lo = 0, hi = 0;
+      int32_t lo = 0, hi = 0;
       const bool in = base + tid < c.batch && rows_of(base + tid, lo, hi);
-      int64_t upto = in ? hi : 0;  // the largest end so far
+      int32_t upto = in ? hi : 0;  // the largest end so far
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t before = __shfl_up_sync(~0u, upto, o);
+        const int32_t before = __shfl_up_sync(~0u, upto, o);
         if ((int)tid >= o) upto = max(upto, before);
       }
-      int64_t before = __shfl_up_sync(~0u, upto, 1);
+      int32_t before = __shfl_up_sync(~0u, upto, 1);
       before = max(taken, tid ? before : 0);
       if (in && lo >= before && has_unit(base + tid, lo, hi)) s_b = (int)(base + tid);
       taken = max(taken, __shfl_sync(~0u, upto, 31));
@@ -684,6 +687,11 @@ __global__ void __launch_bounds__(PK_THREADS) k_kv_pick(SelectArgs a) {
   }
 }
 
+// Units of work of a launch: the rows of its sequences are somewhere among the call's.
+static uint64_t append_units(const grape_kv_cache* cache, uint32_t batch, uint32_t tokens) {
+  return tokens / cache->page_size + 2ull * std::min(AP_BATCH, batch);
+}
+
 static int append_launch(grape_ctx* ctx, const grape_kv_cache* cache, AppendArgs& a, bool interleaved) {
   const uint32_t D = cache->head_dim, KV = cache->kv_heads;
   const uint32_t turned = interleaved ? D / 4 : a.rot / 8 + (D - a.rot) / 4;
@@ -691,9 +699,10 @@ static int append_launch(grape_ctx* ctx, const grape_kv_cache* cache, AppendArgs
   a.plain_items = FastDiv::of(D / 4);
   // Lanes that share an item deal a page's tokens out: more, smaller blocks, until there are eight
   // an SM or a lane would have fewer than eight tokens.
-  const uint64_t units = a.tokens / cache->page_size + 2ull * a.c.batch;
+  const uint32_t batch = a.c.batch;
+  const uint64_t units = append_units(cache, batch, a.tokens);
   const uint64_t items = (uint64_t)KV * turned + (uint64_t)KV * (D / 4) + (uint64_t)a.heads * turned;
-  const uint64_t tokens_per_page = std::min<uint64_t>(cache->page_size, (a.tokens + a.c.batch - 1) / a.c.batch);
+  const uint64_t tokens_per_page = std::min<uint64_t>(cache->page_size, (a.tokens + batch - 1) / batch);
   a.lanes = 1;
   while (a.lanes < 4 && a.lanes * 16 <= tokens_per_page && units * items * a.lanes / AP_THREADS < (uint64_t)ctx->sm_count * 4 * 2) a.lanes *= 2;
   const uint64_t per = AP_THREADS / a.lanes;
@@ -704,9 +713,15 @@ static int append_launch(grape_ctx* ctx, const grape_kv_cache* cache, AppendArgs
   const dim3 grid((uint32_t)units, (uint32_t)chunks);
   auto kernel = cache->bits == 32 ? (interleaved ? k_kv_append<4, true> : k_kv_append<4, false>) : (interleaved ? k_kv_append<2, true> : k_kv_append<2, false>);
   if (int rc = kv_allow_shared(ctx, kernel, ap_smem(interleaved))) return rc;
-  kernel<<<grid, AP_THREADS, ap_smem(interleaved), ctx->stream>>>(a);
-  ctx->launches += 1;
-  GRAPE_CUDA_TRY(ctx, cudaGetLastError());
+  for (uint32_t b = 0; b < batch; b += AP_BATCH) {
+    a.c.batch = std::min(AP_BATCH, batch - b);
+    kernel<<<grid, AP_THREADS, ap_smem(interleaved), ctx->stream>>>(a);
+    ctx->launches += 1;
+    GRAPE_CUDA_TRY(ctx, cudaGetLastError());
+    a.start += AP_BATCH;
+    a.offsets += AP_BATCH;
+    a.c.table += (uint64_t)AP_BATCH * a.c.width;
+  }
   return GRAPE_OK;
 }
 
@@ -788,6 +803,9 @@ extern "C" int grape_kv_append(grape_ctx* ctx, const grape_kv_cache* cache, cons
   if (r.shift > 30 || r.shift + cache->k_shift > 30)
     return kv_refuse(ctx, GRAPE_ERR_INVALID, "rotation shift and key shift add up to more than 30");
   if (tokens > 0x7fffffffu || batch > 0x0fffffffu) return kv_refuse(ctx, GRAPE_ERR_LIMIT, "too many tokens or sequences");
+  const uint64_t launches = ((uint64_t)batch + AP_BATCH - 1) / AP_BATCH;
+  if (launches > 1 && launches * append_units(cache, batch, tokens) > (uint64_t(1) << 30))
+    return kv_refuse(ctx, GRAPE_ERR_LIMIT, "too many sequences and tokens for one call");
   if (batch && (!d_start || !d_offsets || misaligned(d_start, 4) || misaligned(d_offsets, 4)))
     return kv_refuse(ctx, GRAPE_ERR_INVALID, "start and offsets must be given, on 4 bytes");
   const uint64_t row = (uint64_t)cache->kv_heads * cache->head_dim;

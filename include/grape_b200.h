@@ -417,7 +417,8 @@ typedef struct grape_kv_rotation {
  * remainders to d_q_rem / d_k_rem / d_v_rem (dense; any may be NULL).  Slots and bounds of pages that
  * receive nothing stay as they were.  No two sequences of a call may append to the same page.
  * A sequence whose rows begin below 0, run backwards or end behind `tokens` is skipped and sets the status bit;
- * where offsets fall, so is one behind the fall whose rows begin before the end of an earlier one's.
+ * where offsets fall, so is one behind the fall whose rows begin before the end of an earlier one's (of the
+ * same 1024 sequences).  GRAPE_ERR_LIMIT where sequences times pages of tokens pass 2^40.
  * f + k_shift and v_shift are at most 30. */
 int grape_kv_append(grape_ctx* ctx, const grape_kv_cache* cache, const int32_t* d_table, uint32_t table_width,
                     uint32_t batch, const int32_t* d_start, const int32_t* d_offsets, uint32_t tokens,

@@ -83,6 +83,38 @@ def test_append_with_bad_offsets(gctx, offsets, want_taken):
     assert np.array_equal(fetch(gctx, cache.bounds, bounds), bounds)
 
 
+@pytest.mark.parametrize("batch, bits, interleaved", [(4097, 32, True), (9001, 16, False)])
+def test_append_to_very_many_sequences(gctx, batch, bits, interleaved):
+    """None, one or two tokens a sequence, more sequences than a launch takes; one of the last runs outside its table."""
+    from grape_b200 import decode
+    rng = np.random.default_rng(batch)
+    KV, D, page = 1, 16, 8
+    new = rng.integers(0, 3, batch)
+    new[-1], start = 1, rng.integers(0, 6, batch).astype(np.int32)
+    start[-1] = 11                                             # its second page is not there
+    offsets = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    T, table = int(offsets[-1]), rng.permutation(batch).astype(np.int32).reshape(batch, 1)
+    k, v = (Pool(rng, batch, KV, page, D, bits) for _ in range(2))
+    x = rng.integers(-1000, 1000, (T, 2, KV, D)).astype(np.int32)
+    cos, sin = (rng.integers(-65536, 65536, (12, D // 2)).astype(np.int32) for _ in range(2))
+    cache = make_cache(gctx, k, v, page, KV, D, bits)
+    dx, dt, ds, do, dc, dn = (upload(gctx, a) for a in (x, table, start, offsets, cos, sin))
+    gctx.status()
+    decode.kv_append(cache, dt, 1, batch, ds, do, T, dx, dx.at(4 * KV * D), k_stride=2 * KV * D, v_stride=2 * KV * D,
+                     rotation=decode.Rotation(dc, dn, 12, D, interleaved=interleaved))
+    assert gctx.status() == decode.STATUS_PLACE
+    seq = np.repeat(np.arange(batch), new)[:-1]
+    pos = start[seq] + np.arange(T - 1) - offsets[seq]
+    idx = np.arange(D // 2)
+    first, second = (2 * idx, 2 * idx + 1) if interleaved else (idx, idx + D // 2)
+    key, c, s = x[:-1, 0, 0].astype(np.int64), cos[pos].astype(np.int64), sin[pos].astype(np.int64)
+    turned = np.empty_like(key)
+    turned[:, first], turned[:, second] = key[:, first] * c - key[:, second] * s, key[:, second] * c + key[:, first] * s
+    k.view[table[seq, 0], 0, pos] = (turned + (1 << 15)) >> 16
+    v.view[table[seq, 0], 0, pos] = x[:-1, 1, 0]
+    assert np.array_equal(fetch(gctx, cache.k, k.raw), k.raw) and np.array_equal(fetch(gctx, cache.v, v.raw), v.raw)
+
+
 # ---------------------------------------------------------------------------------- select
 @pytest.mark.parametrize("bits", [16, 32])
 @pytest.mark.parametrize("heads, kv_heads, dim", [(4, 1, 3048), (3, 1, 3056), (8, 2, 3064), (2, 1, 4088), (4, 1, 4096)])

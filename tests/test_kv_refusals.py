@@ -154,3 +154,10 @@ def test_python_cache_checks():
         KVCache(None, 1, 16, 1, 64, bits=8)
     with pytest.raises(ValueError):
         KVCache(None, 1, 16, 1, 64, strides=(1024, 1024, 64))
+
+
+def test_append_takes_no_more_work_than_a_call_can_end():
+    """Sequences times pages of tokens: a million of each passes, sixteen million do not."""
+    assert append(cache(), batch=1 << 20, tokens=1 << 20)[1] == "null context"
+    rc, text = append(cache(), batch=1 << 24, tokens=1 << 24)
+    assert rc == 5 and "too many sequences" in text
