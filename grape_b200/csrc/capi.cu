@@ -67,6 +67,7 @@ extern "C" int grape_ctx_destroy(grape_ctx* ctx) {
   if (!ctx) return GRAPE_OK;
   cudaSetDevice(ctx->device);
   cudaStreamSynchronize(ctx->stream);
+  grape::lookups_leave(ctx);
   if (ctx->g_table) grape_table_destroy(ctx->g_table);
   for (auto& b : ctx->arena) cudaFree(b.ptr);
   for (auto& b : ctx->kv_work) cudaFree(b.first);

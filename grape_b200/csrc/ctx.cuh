@@ -10,6 +10,7 @@
 #include "rng.cuh"
 
 struct grape_table;
+struct grape_lookup;
 
 struct grape_ctx {
   int device = 0;
@@ -28,6 +29,7 @@ struct grape_ctx {
   // kept until the context goes, since a captured graph may still hold their addresses.
   std::vector<std::pair<void*, size_t>> kv_work;
   std::vector<const void*> kv_allowed;  // decode-step kernels whose shared memory limit has been raised on this GPU
+  std::vector<grape_lookup*> lookups;   // those of this context that are not destroyed yet
   // pinned staging buffer for the host-buffer entry points
   void* pinned = nullptr;
   size_t pinned_bytes = 0;
@@ -109,6 +111,8 @@ inline void make_device_current(const grape_ctx* ctx) {
   int d = -1;
   if (cudaGetDevice(&d) != cudaSuccess || d != ctx->device) cudaSetDevice(ctx->device);
 }
+
+void lookups_leave(grape_ctx* ctx);  // before a context goes: its lookups no longer know it
 
 inline int fail(grape_ctx* ctx, int code, const std::string& msg) {
   if (ctx) ctx->err = msg;

@@ -287,6 +287,7 @@ static int lookup_create(grape_ctx* ctx, int32_t low, uint32_t len, const int32_
   if (d_map && n != len) return fail(ctx, GRAPE_ERR_INVALID, "lookup: a mapping table must have a power-of-two length");
   grape_lookup* lk = new grape_lookup();
   lk->ctx = ctx;
+  ctx->lookups.push_back(lk);
   lk->low = low;
   lk->n = n;
   lk->mapping = d_map != nullptr;
@@ -345,7 +346,11 @@ extern "C" int grape_lookup_mapping_create(grape_ctx* ctx, int32_t low, uint32_t
 
 extern "C" int grape_lookup_destroy(grape_lookup* lk) {
   if (!lk) return GRAPE_OK;
-  if (lk->ctx) cudaStreamSynchronize(lk->ctx->stream);
+  if (lk->ctx) {
+    cudaStreamSynchronize(lk->ctx->stream);
+    auto& all = lk->ctx->lookups;
+    all.erase(std::remove(all.begin(), all.end(), lk), all.end());
+  }
   cudaFree(lk->T);
   cudaFree(lk->B);
   cudaFree(lk->m);
@@ -357,6 +362,11 @@ extern "C" int grape_lookup_destroy(grape_lookup* lk) {
   }
   delete lk;
   return GRAPE_OK;
+}
+
+// A lookup may outlive its context: it keeps its memory until it is destroyed itself, and nothing else.
+void grape::lookups_leave(grape_ctx* ctx) {
+  for (grape_lookup* lk : ctx->lookups) lk->ctx = nullptr;
 }
 
 extern "C" int grape_lookup_params(const grape_lookup* lk, void* h_alpha, void* h_beta, void* h_r, uint32_t* n) {

@@ -491,8 +491,9 @@ class Lookup:
         if mapped is None:
             ctx._check(ctx.lib.grape_lookup_range_create(ctx.handle, low, length, C.byref(h)))
         else:
-            self._map_dev = ctx.upload(np.ascontiguousarray(mapped, dtype=np.int32))
-            ctx._check(ctx.lib.grape_lookup_mapping_create(ctx.handle, low, length, self._map_dev.ptr, C.byref(h)))
+            d_map = ctx.upload(np.ascontiguousarray(mapped, dtype=np.int32))
+            ctx._check(ctx.lib.grape_lookup_mapping_create(ctx.handle, low, length, d_map.ptr, C.byref(h)))
+            d_map.free()    # the lookup has its own copy
         self.handle = h.value
         a, b, r = (np.zeros((1, 8), dtype=np.uint32) for _ in range(3))
         n = C.c_uint32()
@@ -548,8 +549,8 @@ class Lookup:
         return dict(zip(("A", "S", "B", "T", "m"), vals)), decode_field(u[:n.value])
 
     def close(self):
-        if getattr(self, "handle", None) and self.ctx.handle:    # a context that is gone took its stream along
-            self.ctx.lib.grape_lookup_destroy(self.handle)
+        if getattr(self, "handle", None):
+            self.ctx.lib.grape_lookup_destroy(self.handle)    # knows by itself whether its context is gone
         self.handle = None
 
     def __del__(self):

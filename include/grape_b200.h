@@ -234,6 +234,7 @@ int grape_lookup_range_create(grape_ctx* ctx, int32_t low, uint32_t len, grape_l
  * device memory (len a power of two); draws alpha then r. */
 int grape_lookup_mapping_create(grape_ctx* ctx, int32_t low, uint32_t len, const int32_t* d_map,
                                 grape_lookup** out);
+/* Frees the lookup's memory; also after its context has been destroyed. */
 int grape_lookup_destroy(grape_lookup* lk);
 /* alpha, beta, r (32 bytes each, any may be NULL) and the table size. */
 int grape_lookup_params(const grape_lookup* lk, void* h_alpha, void* h_beta, void* h_r, uint32_t* n);
