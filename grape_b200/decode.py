@@ -170,7 +170,13 @@ class StepProver(LayerProver):
     """Proof of the attention of one new token over one key head, the same walk as a layer's (test/llm.cu:356-452) with
     the heads that share the key head for rows and the cached columns for keys: output remainder, softmax x V, the
     softmax relation, the exp mapping, the score remainder, Q K^T.  What is left are claims on the query, the keys
-    and the values, for the proofs of the tokens that made them."""
+    and the values, for the proofs of the tokens that made them.
+
+    What the walk does not bind, in a layer's proof either: ``exp_in`` to the scores and their row's maximum (any
+    arguments pass whose values, softmax and output go with them), the score remainder to its range (a quotient one
+    larger passes with a remainder ``score_scale`` smaller), and the claim of the softmax relation's range check to the
+    softmax and the exp values it was computed from (of which the latter are opened at its point).  A verifier who needs
+    those links has to make them from the tensors."""
 
     def __init__(self, ctx: Context, shape: StepShape, table, G_jacobian, exp_table):
         for name in ("rows", "keys", "dim"):
@@ -254,6 +260,7 @@ class StepProver(LayerProver):
         trace.lookups += 1
         with self._phase(trace, "lookup"):
             self.softmax_range.prove(resid, rsize, A, e1, table=self.table, msm_size=min(self._n(rsize), self._n(self.softmax_range.n)))
+        self._open(e_out, ssize, e1[:log2ceil(ssize)], self._n(ssize), trace)    # the padding's variables come last
         self._release(resid, tmp, A, soft_keep, e_out)
         consts.free()
         # ---- exp mapping, padded with the table's first pair
