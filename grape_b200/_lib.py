@@ -18,6 +18,7 @@ HEADER = PKG.parent / "include" / "grape_b200.h"
 GRAPE_OK = 0
 ERR_NAMES = {1: "GRAPE_ERR_INVALID", 2: "GRAPE_ERR_CUDA", 3: "GRAPE_ERR_CHECK", 4: "GRAPE_ERR_NOMEM",
              5: "GRAPE_ERR_LIMIT"}
+CUT = 6    # GRAPE_CUT: the call was made, on less than its arguments name
 
 
 class GrapeError(RuntimeError):

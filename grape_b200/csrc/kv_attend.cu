@@ -1343,6 +1343,9 @@ extern "C" int grape_kv_attend(grape_ctx* ctx, const grape_kv_cache* cache, cons
     if (s.sum) s.sum += (uint64_t)b * heads;
     if (int rc = attend_launch(ctx, cache, s)) return rc;
   }
+  if (max_keys < (uint64_t)n_select * cache->page_size)
+    return kv_refuse(ctx, GRAPE_CUT, "max_keys %llu cuts the %llu columns of the selected pages", (unsigned long long)max_keys,
+                     (unsigned long long)n_select * cache->page_size);
   return GRAPE_OK;
 } catch (const std::exception& e) {
   return kv_refuse(nullptr, GRAPE_ERR_NOMEM, "%s", e.what());

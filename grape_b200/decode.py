@@ -12,10 +12,12 @@ call is asynchronous, and what it finds outside the cache, the rotation or the e
 from __future__ import annotations
 
 import ctypes as C
+import warnings
 from dataclasses import dataclass
 
 import numpy as np
 
+from ._lib import CUT
 from .host import FR_MODULUS as R
 from .host import Context, Lookup, _p, decode_field, prove_matmul, reassemble_vectors
 from .layer import FFNTrace, ProofError, log2ceil
@@ -129,13 +131,17 @@ def kv_attend(cache: KVCache, d_table, table_width: int, batch: int, d_len, d_q,
               d_score=None, d_score_rem=None, d_exp_in=None, d_exp_out=None, d_softmax=None, d_sum=None,
               q_stride: int | None = None):
     """``grape_kv_attend``: attention of one token per sequence over its cached positions, or over those of the
-    selected pages, with the tensors of its proof (rows of ``max_keys`` columns)."""
+    selected pages, with the tensors of its proof (rows of ``max_keys`` columns).  Warns where ``max_keys`` cuts the
+    columns of the selected pages, of which the newest come last."""
     ctx = cache.ctx
     w = _Witness(_p(d_score), _p(d_score_rem), _p(d_exp_in), _p(d_exp_out), _p(d_softmax), _p(d_sum), _p(d_out_rem))
-    ctx._check(ctx.lib.grape_kv_attend(ctx.handle, cache._ref, d_table, table_width, batch, d_len, d_selected,
-                                       n_select, d_q, heads * cache.head_dim if q_stride is None else q_stride, heads,
-                                       score_shift, exp.d_values, exp.low, exp.length, soft_shift, max_keys, d_out,
-                                       C.byref(w)))
+    rc = ctx.lib.grape_kv_attend(ctx.handle, cache._ref, d_table, table_width, batch, d_len, d_selected,
+                                 n_select, d_q, heads * cache.head_dim if q_stride is None else q_stride, heads,
+                                 score_shift, exp.d_values, exp.low, exp.length, soft_shift, max_keys, d_out, C.byref(w))
+    if rc == CUT:
+        warnings.warn(ctx.lib.grape_kv_error().decode(), RuntimeWarning, stacklevel=2)
+    else:
+        ctx._check(rc)
 
 
 # ----------------------------------------------------------------------------- proof of a step

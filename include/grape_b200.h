@@ -30,6 +30,7 @@ extern "C" {
 #define GRAPE_ERR_CHECK 3   /* a prover-side round check p(0)+p(1)==claim failed */
 #define GRAPE_ERR_NOMEM 4
 #define GRAPE_ERR_LIMIT 5 /* size beyond a documented fixed limit */
+#define GRAPE_CUT 6       /* not a failure: the call was made, on less than its arguments name (grape_kv_attend) */
 
 #define GRAPE_FR_BYTES 32
 #define GRAPE_AFFINE_BYTES 64
@@ -465,8 +466,11 @@ typedef struct grape_kv_witness {
  * d_exp: exp_len values, not negative, with exp_low <= 0 < exp_low + exp_len.  A score further behind the
  * maximum than the table reaches takes the first entry, and sets a status bit, as does a row of some length
  * whose sum is zero (its softmax and output are zero).  score_shift up to 31, soft_shift 1..20.
- * max_keys bounds the columns of a row: a longer sequence sets a status bit and is cut there.  Columns
- * that hold no position (behind the length, pages outside the cache) are left as they were and weigh
+ * max_keys bounds the columns of a row: a longer sequence sets a status bit and is cut there.  With
+ * d_selected the row is cut there too, and as the lists ascend what is lost are the newest positions: a call
+ * whose max_keys is below n_select * page_size is made and returns GRAPE_CUT in place of GRAPE_OK, with the
+ * text in grape_ctx_error.
+ * Columns that hold no position (behind the length, pages outside the cache) are left as they were and weigh
  * nothing; a row without any position has output, remainder and sum zero.
  * d_out: int32 [batch][heads][head_dim]. */
 int grape_kv_attend(grape_ctx* ctx, const grape_kv_cache* cache, const int32_t* d_table, uint32_t table_width,

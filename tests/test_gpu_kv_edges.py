@@ -1,9 +1,11 @@
 """Calls of the decode step at the edges of what its documentation allows, against plain 64-bit integers."""
+import warnings
+
 import numpy as np
 import pytest
 
-from test_gpu_kv_decode import (WITNESS, Pool, fetch, make_cache, plain_append, plain_attend, plain_select, table_for,
-                                upload)
+from test_gpu_kv_decode import (WITNESS, Pool, exp_table, fetch, make_cache, plain_append, plain_attend, plain_select,
+                                run_attend, table_for, upload)
 
 pytestmark = pytest.mark.gpu
 
@@ -180,3 +182,27 @@ def test_attend_with_the_longest_exp_table(gctx, length, more):
         assert np.array_equal(fetch(gctx, bufs[name], a), a), name
     assert gctx.status() == 0
     exp.free()
+
+
+@pytest.mark.parametrize("length", [70, 4000])
+@pytest.mark.parametrize("missing", [-5, 0, 1, 16])
+def test_columns_of_selected_pages_are_not_cut_without_a_word(gctx, length, missing):
+    """A call whose max_keys is below the columns of the selected pages says so; its outputs are those of the columns before."""
+    rng = np.random.default_rng(length)
+    H, KV, D, page, n = 2, 1, 64, 16, 1 << 20
+    pages = -(-length // page)
+    n_select = min(pages, 150)
+    table = table_for(rng, pages, [length], page)
+    k, v = (Pool(rng, pages, KV, page, D, 32, std=65536) for _ in range(2))
+    q = np.rint(rng.normal(0, 65536, (1, H, D))).astype(np.int32)
+    selected = np.sort(rng.choice(pages - 1, n_select - 1, replace=False)).astype(np.int32)
+    selected = np.append(selected, pages - 1).astype(np.int32).reshape(1, 1, n_select)
+    exp, max_keys = exp_table(n, width=16.0), n_select * page - missing
+    cache = make_cache(gctx, k, v, page, KV, D, 32)
+    want, status = plain_attend(k, v, table, [length], q, exp, 1 - n, page, 19, 16, max_keys, selected=selected)
+    gctx.status()
+    with warnings.catch_warnings(record=True) as said:
+        warnings.simplefilter("always")
+        got, seen = run_attend(gctx, cache, table, [length], q, exp, 1 - n, 19, 16, max_keys, selected=selected)
+    assert [str(w.message) for w in said] == ([f"max_keys {max_keys} cuts the {n_select * page} columns of the selected pages"] if missing > 0 else [])
+    assert seen == status == 0 and all(np.array_equal(got[name], a) for name, a in want.items())
