@@ -81,6 +81,8 @@ class KVCache:
         return buf
 
     def close(self):
+        if self._owned:      # no call may meet the addresses again
+            self._struct.d_k = self._struct.d_v = self._struct.d_bounds = None
         for b in self._owned:
             b.free()
         self._owned = []

@@ -156,6 +156,38 @@ def test_python_cache_checks():
         KVCache(None, 1, 16, 1, 64, strides=(1024, 1024, 64))
 
 
+class NoGpu:
+    """A context's memory without a GPU."""
+    handle = None
+
+    def __init__(self):
+        self.lib, self.next = lib(), 1 << 20
+
+    def alloc(self, nbytes):
+        from grape_b200.host import DeviceBuffer
+        buf = DeviceBuffer.__new__(DeviceBuffer)
+        self.next += -(-nbytes // 256) * 256
+        buf.ctx, buf.nbytes, buf.ptr = self, nbytes, self.next
+        return buf
+
+    def _check(self, rc):
+        pass
+
+
+def test_a_closed_cache_is_refused():
+    """The memory of a cache that allocated it is gone with close(): the calls see a cache without pages."""
+    from grape_b200.decode import KVCache
+    own = KVCache(NoGpu(), 9, 16, 2, 64)
+    assert append(own._struct)[1] == select(own._struct)[1] == attend(own._struct)[1] == "null context"
+    own.close()
+    own.close()
+    assert append(own._struct)[1] == attend(own._struct)[1] == "cache without pages"
+    assert select(own._struct)[1] == "cache without bounds"
+    given = KVCache(NoGpu(), 9, 16, 2, 64, d_k=1 << 20, d_v=1 << 21, d_bounds=1 << 22)
+    given.close()     # the caller's memory is still the caller's
+    assert append(given._struct)[1] == select(given._struct)[1] == "null context"
+
+
 def test_append_takes_no_more_work_than_a_call_can_end():
     """Sequences times pages of tokens: a million of each passes, sixteen million do not."""
     assert append(cache(), batch=1 << 20, tokens=1 << 20)[1] == "null context"
