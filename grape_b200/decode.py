@@ -149,7 +149,8 @@ def kv_attend(cache: KVCache, d_table, table_width: int, batch: int, d_len, d_q,
 # ----------------------------------------------------------------------------- proof of a step
 @dataclass
 class StepShape:
-    """One key head of a step: the heads that share it, the (padded) columns, the head's channels and the scales."""
+    """One key head of a step: the heads that share it, the (padded) columns, the head's channels and the scales.  rows, keys
+    and dim are powers of two, rows * keys and rows * dim at least 16; the three lookups' lengths at least 128."""
     rows: int
     keys: int
     dim: int
@@ -193,6 +194,15 @@ class StepProver(LayerProver):
         exp_table = np.asarray(exp_table, np.int32)
         if exp_table.shape != (shape.exp_len,) or exp_table[0] != 0:
             raise ValueError("the exp table must have exp_len entries, the first of them zero")
+        # an opening takes rows of 16 elements at least, and a lookup commits its multiplicities in rows of 16 sqrt(entries)
+        if min(shape.rows * shape.keys, shape.rows * shape.dim) < 16:
+            raise ValueError("rows * keys and rows * dim must be at least 16: pad the columns")
+        for name in ("scale", "softmax_len", "exp_len"):
+            entries = log2ceil(getattr(shape, name))
+            if entries < 7:
+                raise ValueError(f"{name} must be at least 128")
+            if table.n_gens < 16 << entries // 2:
+                raise ValueError(f"{name} of {getattr(shape, name)} needs a table of {16 << entries // 2} generators, not {table.n_gens}")
         self.step = shape
         self.ctx, self.table, self.G = ctx, table, G_jacobian
         self.shape = LayerShape(layer_num=1, tokens=shape.keys, dim=shape.dim, ffn=shape.dim, scale1=shape.scale, npoints=shape.dim)

@@ -63,3 +63,29 @@ def test_exp_arguments_are_not_tied_to_the_scores(gctx, step):  # noqa: F811
     assert not np.array_equal(quotient, t["qkv_q"])
     t["qkv_q"], t["qkv_rem"] = quotient.astype(np.int32), (acc - quotient * shape.scale).astype(np.int32)
     proven(gctx, shape, exp, t, 9)
+
+
+@pytest.mark.parametrize("rows, cached, keys, dim, exp_len, softmax_len", [
+    (1, 1, 16, 16, 128, 128), (16, 1, 1, 1, 512, 128), (2, 1, 8, 8, 512, 128), (1, 200, 256, 64, 512, 4096), (8, 300, 512, 64, 512, 8192),
+    (1, 16, 16, 4096, 128, 1024), (4096, 1, 1, 1, 128, 128)])
+def test_the_smallest_steps_and_lopsided_ones(gctx, rows, cached, keys, dim, exp_len, softmax_len):
+    """A first token, one head, one channel, many heads: every claim that is left holds."""
+    from grape_b200 import decode
+    rng = np.random.default_rng(rows + keys + dim)
+    q, k, v = (np.rint(rng.normal(0, 64, s)).astype(np.int64) for s in ((rows, dim), (cached, dim), (cached, dim)))
+    exp = np.rint(7 * np.exp(-np.arange(exp_len)[::-1] * 9 / exp_len)).astype(np.int32)
+    exp[0] = 0
+    acc = q @ k.T
+    score = (acc + 256) >> 9
+    exp_in = np.maximum(score - score.max(axis=1, keepdims=True), 1 - exp_len)
+    exp_out = exp[exp_in - (1 - exp_len)].astype(np.int64)
+    total = exp_out.sum(axis=1, keepdims=True)
+    assert 2 * total.max() <= softmax_len
+    softmax = ((exp_out << 8) + total // 2) // total
+    product = softmax @ v
+    out = (product + 128) >> 8
+    shape = decode.StepShape(rows=rows, keys=keys, dim=dim, scale=1 << 8, score_scale=1 << 9, exp_low=1 - exp_len, exp_len=exp_len,
+                             softmax_len=softmax_len)
+    t = decode.pad_step(shape, q, k, v, {"score": score, "score_rem": acc - (score << 9), "exp_in": exp_in, "exp_out": exp_out,
+                                         "softmax": softmax, "out": out, "out_rem": product - (out << 8)})
+    proven(gctx, shape, exp, t, 11)

@@ -188,6 +188,21 @@ def test_a_closed_cache_is_refused():
     assert append(given._struct)[1] == select(given._struct)[1] == "null context"
 
 
+@pytest.mark.parametrize("change, gens, word", [
+    (dict(keys=1), 16384, "pad the columns"), (dict(rows=2, dim=4), 16384, "pad the columns"), (dict(scale=64), 16384, "scale"),
+    (dict(softmax_len=64), 16384, "softmax_len"), (dict(exp_len=64), 16384, "exp_len"), (dict(), 1024, "scale of 65536"),
+    (dict(softmax_len=1 << 18), 4096, "8192 generators"), (dict(exp_len=1 << 20), 4096, "16384 generators")])
+def test_steps_that_cannot_be_proven(change, gens, word):
+    """Shapes that an opening or a lookup would refuse in the middle of a proof are refused before it."""
+    from types import SimpleNamespace
+
+    import numpy as np
+    from grape_b200.decode import StepProver, StepShape
+    shape = StepShape(**{**dict(rows=1, keys=16, dim=64, exp_len=512, exp_low=-511), **change})
+    with pytest.raises(ValueError, match=word):
+        StepProver(None, shape, SimpleNamespace(n_gens=gens), None, np.zeros(shape.exp_len, np.int32))
+
+
 def test_append_takes_no_more_work_than_a_call_can_end():
     """Sequences times pages of tokens: a million of each passes, sixteen million do not."""
     assert append(cache(), batch=1 << 20, tokens=1 << 20)[1] == "null context"
