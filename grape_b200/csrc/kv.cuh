@@ -8,7 +8,7 @@
 
 namespace grape {
 
-// n / d for 0 <= n < 2^31 by one high product (d >= 1): with l = ceil(log2 d) and
+// n / d by one high product (d >= 1; Granlund and Montgomery's division by invariant integers): with l = ceil(log2 d) and
 // m = floor(2^32 (2^l - d) / d) + 1 the quotient is (hi(m n) + n) >> l.
 struct FastDiv {
   uint32_t d, m, l;
@@ -60,6 +60,16 @@ __device__ __forceinline__ int32_t saturate(int64_t x, int64_t low, int64_t high
   if (x > high) { out_of_range = true; return (int32_t)high; }
   return (int32_t)x;
 }
+
+// Asynchronous copies into a lane's own queue in shared memory.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // ---- host side ---------------------------------------------------------------------------------
 int kv_refuse(grape_ctx* ctx, int code, const char* format, ...);

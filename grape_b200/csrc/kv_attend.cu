@@ -145,16 +145,6 @@ __device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.
 // SM have under way (about 150 KB) is what carries the kernels: one step at a time in registers (64 KB) gave
 // 3 TB/s.  Whole rows by bulk copies of one warp for all gave 3.4 TB/s, the same copies by a warp's lanes 3.1 to
 // 4.3: the issuing warps could not keep up.
-__device__ __forceinline__ void copy_async(void* to, const char* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy_async_8(void* to, const unsigned char* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ void mma_u8s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
@@ -305,7 +295,7 @@ __global__ void __launch_bounds__(MT == 2 ? 256 : 512) k_kv_scores(AttendArgs a)
       }
       if (ahead_blk * 64 + t * 16 < row_bytes) {
 #pragma unroll
-        for (int m = 0; m < 2 * MT; m++) copy_async(queue + (ahead_stage * 2 * MT + m) * 32, key[m] + ahead_blk * 64);
+        for (int m = 0; m < 2 * MT; m++) copy_async<16>(queue + (ahead_stage * 2 * MT + m) * 32, key[m] + ahead_blk * 64);
       }
       ahead_stage = ahead_stage + 1 == STAGES ? 0 : ahead_stage + 1;
       if (++ahead_blk == blk1) {
@@ -738,8 +728,8 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
   settle();
   auto fetch_digits = [&](char* to, const unsigned char* from, bool has) {
     if (has) {
-      copy_async_8(to + my_digits, from);
-      if (NT == 2 && col_digit == 0) copy_async_8(to + my_digits + 256, from + 2 * a.padded);
+      copy_async<8>(to + my_digits, from);
+      if (NT == 2 && col_digit == 0) copy_async<8>(to + my_digits + 256, from + 2 * a.padded);
     }
   };
   auto fetch = [&](bool with_digits) {
@@ -750,7 +740,7 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
         if (ahead_in) {
 #pragma unroll
           for (int j = 0; j < 8; j++) {
-            copy_async(to + my_rows + j * 512, from);
+            copy_async<16>(to + my_rows + j * 512, from);
             from += c.slot_stride;
           }
         }
@@ -758,7 +748,7 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           const int64_t row = __shfl_sync(~0u, next_row, 8 * t + j);
-          if (ahead_in) copy_async(to + my_rows + j * 512, ahead_base + row);
+          if (ahead_in) copy_async<16>(to + my_rows + j * 512, ahead_base + row);
         }
       }
       if (with_digits) fetch_digits(to, ahead_digits, ahead_has);
@@ -934,7 +924,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_kv_small(AttendArgs a) {
       if (ahead_set < sets) {
         if (ahead_blk * 64 + t * 16 < row_bytes) {
 #pragma unroll
-          for (int m = 0; m < 4; m++) copy_async(queue + (ahead_stage * 4 + m) * 32, c.k + s_row[ahead_set * 32 + m * 8 + gl] + ahead_blk * 64 + t * 16);
+          for (int m = 0; m < 4; m++) copy_async<16>(queue + (ahead_stage * 4 + m) * 32, c.k + s_row[ahead_set * 32 + m * 8 + gl] + ahead_blk * 64 + t * 16);
         }
         ahead_stage = ahead_stage + 1 == SM_STAGES ? 0 : ahead_stage + 1;
         if (++ahead_blk == blks) {
@@ -1024,7 +1014,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_kv_small(AttendArgs a) {
     if (ahead < sets) {
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        if (byte < row_bytes) copy_async(mine + ahead_stage * 4096 + my_rows + j * 512, c.v + s_row[ahead * 32 + 8 * t + j] + byte);
+        if (byte < row_bytes) copy_async<16>(mine + ahead_stage * 4096 + my_rows + j * 512, c.v + s_row[ahead * 32 + 8 * t + j] + byte);
       ahead_stage = ahead_stage + 1 == SM_VALUE_STAGES ? 0 : ahead_stage + 1;
       ahead += teams;
     }

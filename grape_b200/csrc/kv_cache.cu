@@ -131,15 +131,6 @@ struct AppendArgs {
 __host__ __device__ constexpr int ap_stages(bool interleaved) { return interleaved ? 8 : 6; }
 constexpr size_t ap_smem(bool interleaved) { return (size_t)ap_stages(interleaved) * AP_THREADS * (interleaved ? 32 : 64); }
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const int32_t* from) {
-  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 template <int EB, bool INTERLEAVED>
 __global__ void __launch_bounds__(AP_THREADS, INTERLEAVED ? 3 : 2) k_kv_append(AppendArgs a) {
   __shared__ int s_b;
