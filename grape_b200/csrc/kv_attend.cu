@@ -443,6 +443,7 @@ __global__ void __launch_bounds__(MT == 2 ? 256 : 512) k_kv_scores(AttendArgs a)
 // prover's) lives in L2; a thread has four columns under way, since what it waits for is a chain of loads.
 constexpr uint32_t EX_COLS = 4, EX_MAX_THREADS = 1024;
 
+// Two blocks of 1024 threads an SM leave 32 registers, of which 20 to 28 bytes spill.
 // A warp takes 128 columns at a time, a lane four that lie together where the rows of the witness begin on 16 bytes
 // (ALIGNED: one access each), else every 32nd.
 template <bool ALIGNED>
@@ -669,7 +670,8 @@ __device__ __forceinline__ void multiply_step(int32_t (&acc)[8][NT][4], const ch
   }
 }
 
-// NH: heads of a warp, 1, 2 or 4.  A block takes a.v_heads = NH or 8.
+// NH: heads of a warp, 1, 2 or 4.  A block takes a.v_heads = NH or 8.  Two blocks an SM leave 128 registers: with four heads
+// 86 bytes a thread spill with 32-bit values and 158 with 16.
 template <int EB, int NH>
 __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
   constexpr int NT = NH == 4 ? 2 : 1;      // columns of a warp in eights
@@ -848,7 +850,7 @@ __global__ void __launch_bounds__(VA_THREADS, 2) k_kv_values(AttendArgs a) {
 // and their beginnings cost more than the bytes.  Scores, softmax and digits stay in shared memory between the
 // passes; the arithmetic is that of the passes above.
 // Measured against the three passes (us): 32 caches of 64 / 256 / 512 keys, 32 heads on 8 of 128: 15 / 29 / 44 against
-// 31 / 47 / 62; 4 caches of 512: 25 against 27; one cache of 256, 4 heads of 64: 14 against 23.  With few rows and
+// 31 / 47 / 62 (their bytes alone 3 / 11 / 22); 4 caches of 512: 25 against 27; one cache of 256, 4 heads of 64: 14 against 23.  With few rows and
 // long ones a block alone is too slow: 2 caches of 1024 keys of 16 bits, 16 heads on 4: 31 against 25.
 constexpr uint32_t SM_BYTES = 256 * 1024;     // keys of a row at most
 constexpr uint32_t SM_BYTES_FEW = 128 * 1024; // where there are fewer than SM_MANY blocks

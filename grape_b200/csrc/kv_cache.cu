@@ -405,7 +405,8 @@ __global__ void __launch_bounds__(AP_THREADS, INTERLEAVED ? 3 : 2) k_kv_append(A
 // time reached 2.1 TB/s; eight, for one head, leave room for fewer warps: 48 us where four take 35), and four pages
 // x four heads of sums to add up over the lanes, each step of which halves what a lane holds: 32 shuffles for
 // 16 sums where one sum after the other takes 160.
-// What bounds it: bytes of the bounds; a channel and head costs one select and one wide multiply-add.
+// What bounds it: bytes of the bounds, fetched again for every four heads; a channel and head costs one select and one
+// wide multiply-add.
 constexpr int SB_THREADS = 128;
 constexpr int SB_PAGES = 4;  // whose sums a lane holds at a time, for up to four heads
 

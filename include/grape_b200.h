@@ -373,7 +373,7 @@ const char* grape_static_error(void);
  * rdiv(x, s) below is the rounded division by 2^s: floor((x + floor(2^s / 2)) / 2^s); the remainder
  * x - rdiv(x, s) * 2^s lies in [-2^(s-1), 2^(s-1)).
  * All products and sums are 64-bit integers, so every output is exact and does not depend on how the
- * work is split; inputs have to keep |q . k| and |x cos| + |x sin| below 2^63.  A quotient that does not
+ * work is split; inputs have to keep |q . k|, a page's bound and |x cos| + |x sin| below 2^63.  A quotient that does not
  * fit its type is stored as the type's nearest value and sets a status bit (grape_ctx_status).
  * Device data (lengths, page numbers, positions) is checked on the device: what points outside the
  * cache, the table or the rotation is skipped and sets a status bit, nothing is read or written there.
